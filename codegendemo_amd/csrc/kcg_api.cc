@@ -33,6 +33,7 @@
 #include <vector>
 
 #include "kcg_config.h"
+#include "kcg_host.h"
 
 #define KCG_VERSION "kcg-gemm-gfx950 0.3"
 
@@ -122,6 +123,8 @@ int fail(int code, const std::string& msg) {
 
 #define KCG_HIP_FUNCS(X)      \
   X(hipSetDevice)             \
+  X(hipGetDevice)             \
+  X(hipGetDeviceCount)        \
   X(hipModuleLoadData)        \
   X(hipModuleGetFunction)     \
   X(hipModuleUnload)          \
@@ -415,6 +418,24 @@ int copy_out(const std::string& s, char* out, int out_len) {
 }
 
 }  // namespace
+
+namespace kcg {
+
+int host_fail(int code, const std::string& msg) { return fail(code, msg); }
+int host_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+void host_clear_error() { g_err.clear(); }
+const HostHip* host_hip() {
+  if (!hip_api().ok) {
+    fail(KCG_ERR_HIP, "KCG Error[HIP]: runtime unavailable:" + hip_api().error);
+    return nullptr;
+  }
+  static const HostHip h = {HIPF(hipGetDevice),       HIPF(hipSetDevice),         HIPF(hipGetDeviceCount),
+                            HIPF(hipModuleLoadData),  HIPF(hipModuleGetFunction), HIPF(hipModuleUnload),
+                            HIPF(hipModuleLaunchKernel), hip_api().p_hipFuncSetAttribute};
+  return &h;
+}
+
+}  // namespace kcg
 
 extern "C" {
 

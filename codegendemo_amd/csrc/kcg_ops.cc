@@ -1,0 +1,303 @@
+// kcg_ops.cc — host side of the operators declared in include/kcg_ops.h: argument checks, the choice of a kernel, launches.
+#include <climits>
+#include <cstring>
+#include <map>
+#include <memory>
+#include <mutex>
+#include <string>
+
+#include "../../include/kcg_gemm.h"
+#include "../../include/kcg_ops.h"
+#include "kcg_host.h"
+#include "kcg_ops_args.h"
+
+// the code object of kcg_ops.hip
+__asm__(".section .rodata\n.balign 4096\n.global kcg_ops_code\nkcg_ops_code:\n.incbin \"" KCG_OPS_CODE "\"\n.byte 0\n.previous\n");
+extern "C" const char kcg_ops_code[];
+
+namespace {
+
+using kcg::host_fail;
+using kcg::host_hip;
+using kcg::host_hip_fail;
+using kcg::HostHip;
+using namespace kcg_ops;
+
+// ---- kernels ---------------------------------------------------------------------------------
+enum { kNorm = 0, kSwiglu = kNorm + 21, kSkinny = kSwiglu + 3, kTile = kSkinny + 9, kMoeUp = kTile + 8, kMoeDown = kMoeUp + 3, kNumKernels = kMoeDown + 3 };
+
+std::string kernel_symbol(int i) {
+  static const char* const types[3] = {"bf16", "f16", "f32"};
+  static const char* const norm[7] = {"64_1", "128_1", "256_1", "512_1", "1024_1", "1024_2", "1024_0"};
+  static const char* const tile[8] = {"bf16_256x256", "f16_256x256", "bf16_128x128", "f16_128x128", "f32_128x128", "bf16_64x64", "f16_64x64", "f32_64x64"};
+  static const char* const moe[3] = {"e4m3_bf16", "e4m3_f16", "bf16_bf16"};
+  if (i < kSwiglu) return std::string("kcg_norm_") + types[i / 7] + "_" + norm[i % 7];
+  if (i < kSkinny) return std::string("kcg_swiglu_") + types[i - kSwiglu];
+  if (i < kTile) return std::string("kcg_mm8_skinny_") + types[(i - kSkinny) / 3] + "_" + std::to_string(1 << (i - kSkinny) % 3);
+  if (i < kMoeUp) return std::string("kcg_mm8_tile_") + tile[i - kTile];
+  if (i < kMoeDown) return std::string("kcg_moe_up_") + moe[i - kMoeUp];
+  return std::string("kcg_moe_down_") + moe[i - kMoeDown];
+}
+
+struct DeviceKernels {
+  hipModule_t module;
+  hipFunction_t fn[kNumKernels];
+};
+
+// `device` current while it lives, the caller's device again afterwards
+struct OnDevice {
+  const HostHip* hip;
+  int before = -1;
+  hipError_t error;
+  OnDevice(const HostHip* h, int device) : hip(h) {
+    int now = -1;
+    error = hip->GetDevice(&now);
+    if (error == hipSuccess && now != device) {
+      error = hip->SetDevice(device);
+      if (error == hipSuccess) before = now;
+    }
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hip->SetDevice(before);
+  }
+};
+
+int moe_partial_bytes(int64_t tokens, int64_t topk) { return (int)(tokens * (topk > 16 ? topk : 16) * 16 * 4); }
+
+// The kernels on `device` (current): loaded once per process and device, kept until the process ends.
+int kernels_on(const HostHip* hip, int device, const DeviceKernels** out) {
+  static std::mutex mu;
+  static std::map<int, std::unique_ptr<DeviceKernels>> loaded;
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = loaded.find(device);
+  if (it == loaded.end()) {
+    std::unique_ptr<DeviceKernels> k(new DeviceKernels);
+    hipError_t e = hip->ModuleLoadData(&k->module, kcg_ops_code);
+    if (e != hipSuccess) return host_hip_fail(e, "hipModuleLoadData (operators)");
+    for (int i = 0; i < kNumKernels && e == hipSuccess; ++i) {
+      e = hip->ModuleGetFunction(&k->fn[i], k->module, kernel_symbol(i).c_str());
+      // a block of the experts' second kernel may use more than 64 KiB of LDS, part of it dynamic
+      if (e == hipSuccess && i >= kMoeDown)
+        e = hip->FuncSetAttribute ? hip->FuncSetAttribute((const void*)k->fn[i], hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                          moe_partial_bytes(MOE_T, MOE_K))
+                                  : hipErrorNotSupported;
+    }
+    if (e != hipSuccess) {
+      (void)hip->ModuleUnload(k->module);
+      return host_hip_fail(e, "hipModuleGetFunction (operators)");
+    }
+    it = loaded.emplace(device, std::move(k)).first;
+  }
+  *out = it->second.get();
+  return KCG_OK;
+}
+
+int launch(const HostHip* hip, hipFunction_t fn, unsigned gx, unsigned gy, unsigned block, unsigned lds, uint64_t stream, void* args) {
+  void* params[1] = {args};
+  const hipError_t e = hip->ModuleLaunchKernel(fn, gx, gy, 1, block, 1, 1, lds, (hipStream_t)(uintptr_t)stream, params, nullptr);
+  return e == hipSuccess ? (int)KCG_OK : host_hip_fail(e, "hipModuleLaunchKernel");
+}
+
+// runs f(hip, kernels) with `device` current; nothing is thrown past it
+template <class F>
+int on_device(int device, F f) {
+  try {
+    const HostHip* hip = host_hip();
+    if (!hip) return KCG_ERR_HIP;
+    OnDevice guard(hip, device);
+    if (guard.error != hipSuccess) return host_hip_fail(guard.error, "hipSetDevice");
+    const DeviceKernels* k = nullptr;
+    if (int rc = kernels_on(hip, device, &k)) return rc;
+    const int rc = f(hip, *k);
+    if (rc == KCG_OK) kcg::host_clear_error();
+    return rc;
+  } catch (...) {
+    return KCG_ERR_HIP;      // out of host memory while a message or a table was made
+  }
+}
+
+int bad(const char* what) {
+  try {
+    return host_fail(KCG_ERR_ARGUMENT, what);
+  } catch (...) {
+    return KCG_ERR_ARGUMENT;
+  }
+}
+
+// ---- checks ------------------------------------------------------------------------------------
+int type_index(int64_t dtype) { return dtype == KCG_DT_BFLOAT16 ? 0 : dtype == KCG_DT_FLOAT16 ? 1 : dtype == KCG_DT_FLOAT32 ? 2 : -1; }
+int type_bytes(int64_t dtype) { return dtype == KCG_DT_FLOAT32 ? 4 : dtype == KCG_DT_E4M3 ? 1 : 2; }
+constexpr int64_t kMaxExtent = 1 << 30;       // rows and columns: 32-bit indices in the kernels, with room for a tile
+constexpr int64_t kMaxStride = (int64_t)1 << 40;
+bool extent_ok(int64_t n) { return n >= 0 && n <= kMaxExtent; }
+// a row stride: rows do not overlap (any value goes where there is one row)
+bool stride_ok(int64_t stride, int64_t cols, int64_t rows) { return stride >= 0 && stride <= kMaxStride && (rows <= 1 || stride >= cols); }
+bool any_stride_ok(int64_t s) { return s >= 0 && s <= kMaxStride; }
+bool aligned(int64_t p, int64_t to) { return p % to == 0; }
+int64_t groups(int64_t n) { return (n + 127) / 128; }
+
+// output scales [rows, groups]: no two of them in one place
+bool scale_layout_ok(int64_t row, int64_t group, int64_t rows, int64_t ng) {
+  if (!any_stride_ok(row) || !any_stride_ok(group)) return false;
+  if (rows > 1 && row == 0) return false;
+  if (ng > 1 && group == 0) return false;
+  if (rows > 1 && ng > 1) return row >= group * ng || group >= row * rows;
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kcg_ops_load(int device) {
+  return on_device(device, [](const HostHip*, const DeviceKernels&) { return (int)KCG_OK; });
+}
+
+int kcg_rmsnorm_quant(const kcg_rmsnorm_quant_args* p, int device, uint64_t stream) {
+  if (!p) return bad("rmsnorm_quant: null argument");
+  const int t = type_index(p->dtype);
+  if (t < 0) return bad("rmsnorm_quant: x must be bfloat16, float16 or float32");
+  if (p->weight_dtype != p->dtype && p->weight_dtype != KCG_DT_FLOAT32) return bad("rmsnorm_quant: the weight must have x's type or float32");
+  if (!extent_ok(p->rows) || !extent_ok(p->cols)) return bad("rmsnorm_quant: rows and cols must be in [0, 2^30]");
+  if (!(p->eps >= 0)) return bad("rmsnorm_quant: eps must not be negative");
+  if (!p->residual != !p->residual_out) return bad("rmsnorm_quant: residual and residual_out go together");
+  if (p->rows == 0 || p->cols == 0) return KCG_OK;
+  if (!p->x || !p->weight || !p->q || !p->scale) return bad("rmsnorm_quant: null device pointer");
+  const int es = type_bytes(p->dtype);
+  if (!aligned(p->x, es) || !aligned(p->residual, es) || !aligned(p->residual_out, es) || !aligned(p->y, es) ||
+      !aligned(p->weight, type_bytes(p->weight_dtype)) || !aligned(p->scale, 4))
+    return bad("rmsnorm_quant: an address is not aligned to its elements");
+  if (!aligned(p->q, 16) || (p->rows > 1 && !aligned(p->q_stride, 16))) return bad("rmsnorm_quant: rows of q must start on 16 bytes");
+  if (!stride_ok(p->x_stride, p->cols, 1) || !stride_ok(p->q_stride, p->cols, p->rows) || (p->y && !stride_ok(p->y_stride, p->cols, p->rows)) ||
+      (p->residual && (!stride_ok(p->residual_stride, p->cols, 1) || !stride_ok(p->residual_out_stride, p->cols, p->rows))))
+    return bad("rmsnorm_quant: a row stride is negative or smaller than a row");
+  if (!scale_layout_ok(p->scale_stride_row, p->scale_stride_group, p->rows, groups(p->cols))) return bad("rmsnorm_quant: scales overlap");
+  NormArgs a = {(const void*)p->x, (const void*)p->residual, (void*)p->residual_out, (const void*)p->weight, (void*)p->y, (uint8_t*)p->q, (float*)p->scale,
+                p->x_stride, p->residual_stride, p->residual_out_stride, p->y_stride, p->q_stride, p->scale_stride_row, p->scale_stride_group,
+                (int)p->rows, (int)p->cols, p->weight_dtype == KCG_DT_FLOAT32, (float)p->eps};
+  // threads per row: one vector of 8 each, up to 1024; two each up to 16384 columns; beyond, the row is read twice
+  const int64_t nv = (p->cols + 7) / 8;
+  const int v = nv <= 64 ? 0 : nv <= 128 ? 1 : nv <= 256 ? 2 : nv <= 512 ? 3 : nv <= 1024 ? 4 : nv <= 2048 ? 5 : 6;
+  static const int threads[7] = {256, 128, 256, 512, 1024, 1024, 1024};
+  const int64_t blocks = v == 0 ? (p->rows + 3) / 4 : p->rows;
+  return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) {
+    return launch(hip, k.fn[kNorm + t * 7 + v], (unsigned)blocks, 1, threads[v], 0, stream, &a);
+  });
+}
+
+int kcg_swiglu_quant(const kcg_swiglu_quant_args* p, int device, uint64_t stream) {
+  if (!p) return bad("swiglu_quant: null argument");
+  const int t = type_index(p->dtype);
+  if (t < 0) return bad("swiglu_quant: gate_up must be bfloat16, float16 or float32");
+  if (!extent_ok(p->rows) || !extent_ok(p->cols)) return bad("swiglu_quant: rows and cols must be in [0, 2^30]");
+  if (p->rows == 0 || p->cols == 0) return KCG_OK;
+  if (!p->gate_up || !p->q || !p->scale) return bad("swiglu_quant: null device pointer");
+  if (!aligned(p->gate_up, type_bytes(p->dtype)) || !aligned(p->scale, 4)) return bad("swiglu_quant: an address is not aligned to its elements");
+  if (!aligned(p->q, 16) || (p->rows > 1 && !aligned(p->q_stride, 16))) return bad("swiglu_quant: rows of q must start on 16 bytes");
+  if (!stride_ok(p->gate_up_stride, 2 * p->cols, 1) || !stride_ok(p->q_stride, p->cols, p->rows))
+    return bad("swiglu_quant: a row stride is negative or smaller than a row");
+  if (!scale_layout_ok(p->scale_stride_row, p->scale_stride_group, p->rows, groups(p->cols))) return bad("swiglu_quant: scales overlap");
+  const int64_t threads = p->rows * groups(p->cols) * 16;
+  if (threads > (int64_t)UINT_MAX - 256) return bad("swiglu_quant: rows * cols is too large");
+  SwigluArgs a = {(const void*)p->gate_up, (uint8_t*)p->q, (float*)p->scale, p->gate_up_stride, p->q_stride, p->scale_stride_row, p->scale_stride_group,
+                  (unsigned)p->rows, (int)p->cols};
+  return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) {
+    return launch(hip, k.fn[kSwiglu + t], (unsigned)((threads + 255) / 256), 1, 256, 0, stream, &a);
+  });
+}
+
+int kcg_matmul_fp8(const kcg_matmul_fp8_args* p, int device, uint64_t stream) {
+  if (!p) return bad("matmul_fp8: null argument");
+  const int t = type_index(p->c_dtype);
+  if (t < 0) return bad("matmul_fp8: c must be bfloat16, float16 or float32");
+  if (!extent_ok(p->m) || !extent_ok(p->n) || !extent_ok(p->k)) return bad("matmul_fp8: m, n and k must be in [0, 2^30]");
+  if (p->m == 0 || p->n == 0) return KCG_OK;
+  if (!p->c || (p->k > 0 && (!p->a || !p->a_scale || !p->b || !p->b_scale))) return bad("matmul_fp8: null device pointer");
+  const int es = type_bytes(p->c_dtype);
+  if (!aligned(p->c, es) || !aligned(p->a_scale, 4) || !aligned(p->b_scale, 4)) return bad("matmul_fp8: an address is not aligned to its elements");
+  if (p->k > 0 && (!aligned(p->a, 16) || !aligned(p->b, 16) || (p->m > 1 && !aligned(p->a_stride, 16)) || (p->n > 1 && !aligned(p->b_stride, 16))))
+    return bad("matmul_fp8: rows of a and b must start on 16 bytes");
+  if (!stride_ok(p->a_stride, p->k, p->m) || !stride_ok(p->b_stride, p->k, p->n) || !stride_ok(p->c_stride, p->n, p->m))
+    return bad("matmul_fp8: a row stride is negative or smaller than a row");
+  if (!any_stride_ok(p->a_scale_stride_row) || !any_stride_ok(p->a_scale_stride_group) || !any_stride_ok(p->b_scale_stride_row) ||
+      !any_stride_ok(p->b_scale_stride_group))
+    return bad("matmul_fp8: a stride of the scales is negative");
+  // a tile addresses its rows with 32-bit offsets from its first one
+  if ((p->m > 1 && p->a_stride > (1 << 22)) || (p->n > 1 && p->b_stride > (1 << 22)) || (p->m > 1 && p->a_scale_stride_row > (1 << 20)))
+    return bad("matmul_fp8: rows of a, b or a_scale are more than 2^22 (2^20) elements apart");
+  MatmulArgs a = {(const uint8_t*)p->a, (const uint8_t*)p->b, (const float*)p->a_scale, (const float*)p->b_scale, (void*)p->c,
+                  p->m > 1 ? p->a_stride : 0, p->n > 1 ? p->b_stride : 0, p->c_stride, p->m > 1 ? p->a_scale_stride_row : 0, p->a_scale_stride_group,
+                  p->b_scale_stride_row, p->b_scale_stride_group, (int)p->m, (int)p->n, (int)p->k, (int)groups(p->k), 0, 0, 0};
+  a.c_wide = aligned(p->c, 4 * es) && (p->m == 1 || aligned(p->c_stride, 4));
+  int fn, block;
+  int64_t blocks;
+  if (p->m <= 64) {
+    fn = kSkinny + t * 3 + (p->m <= 16 ? 0 : p->m <= 32 ? 1 : 2);
+    block = 512;
+    blocks = (p->n + 15) / 16;
+  } else {
+    static const int edge[3] = {256, 128, 64}, threads[3] = {512, 256, 256};
+    static const int first[3] = {kTile, kTile + 2, kTile + 5};
+    int v = t == 2 ? 1 : 0;                // (float32 results: the wide operands of a 256 x 256 tile do not fit the registers)
+    for (; v < 2; ++v)
+      if (((p->m + edge[v] - 1) / edge[v]) * ((p->n + edge[v] - 1) / edge[v]) >= 192) break;
+    a.grid_m = (int)((p->m + edge[v] - 1) / edge[v]);
+    a.grid_n = (int)((p->n + edge[v] - 1) / edge[v]);
+    blocks = (int64_t)a.grid_m * a.grid_n;
+    fn = first[v] + t;
+    block = threads[v];
+  }
+  if (blocks > (1 << 30)) return bad("matmul_fp8: m * n is too large");
+  return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) { return launch(hip, k.fn[fn], (unsigned)blocks, 1, block, 0, stream, &a); });
+}
+
+int64_t kcg_moe_workspace_bytes(int64_t tokens, int64_t experts, int64_t topk, int64_t hidden, int64_t inter) {
+  if (tokens < 0 || tokens > MOE_T) return bad("moe_layer: tokens must be in [0, 64] (this is the layer for a few tokens)");
+  if (experts < 1 || experts > MOE_E) return bad("moe_layer: experts must be in [1, 512]");
+  if (topk < 1 || topk > MOE_K || topk > experts) return bad("moe_layer: topk must be in [1, 16] and at most experts");
+  if (hidden < 16 || hidden % 16 || hidden > (1 << 20) || inter < 16 || inter % 16 || inter > (1 << 20))
+    return bad("moe_layer: hidden and inter must be multiples of 16, at most 2^20");
+  const int64_t slots = tokens * topk < experts ? tokens * topk : experts;
+  const int64_t bytes = 2 * (tokens * topk * inter * 2) + slots * MOE_SLOT * 4 + tokens * topk * 4;
+  return (bytes + 15) / 16 * 16;
+}
+
+int kcg_moe_layer(const kcg_moe_layer_args* p, int device, uint64_t stream) {
+  if (!p) return bad("moe_layer: null argument");
+  const int64_t need = kcg_moe_workspace_bytes(p->tokens, p->experts, p->topk, p->hidden, p->inter);
+  if (need < 0) return (int)need;
+  int v;
+  if (p->weight_dtype == KCG_DT_E4M3 && p->dtype == KCG_DT_BFLOAT16) v = 0;
+  else if (p->weight_dtype == KCG_DT_E4M3 && p->dtype == KCG_DT_FLOAT16) v = 1;
+  else if (p->weight_dtype == KCG_DT_BFLOAT16 && p->dtype == KCG_DT_BFLOAT16) v = 2;
+  else return bad("moe_layer: weights in e4m3 with x in bfloat16 or float16, or both in bfloat16");
+  if (p->tokens == 0) return KCG_OK;
+  if (!p->x || !p->logits || !p->w13 || !p->w2 || !p->out || !p->ids || !p->probs || !p->workspace) return bad("moe_layer: null device pointer");
+  if (v != 2 && (!p->w13_scale || !p->w2_scale)) return bad("moe_layer: e4m3 weights need their scales");
+  if (p->workspace_bytes < need) return bad("moe_layer: the workspace is smaller than kcg_moe_workspace_bytes says");
+  if (!aligned(p->x, 2) || !aligned(p->out, 2) || !aligned(p->logits, 4) || !aligned(p->ids, 4) || !aligned(p->probs, 4) || !aligned(p->w13_scale, 4) ||
+      !aligned(p->w2_scale, 4))
+    return bad("moe_layer: an address is not aligned to its elements");
+  const int64_t wb = type_bytes(p->weight_dtype), per16 = 16 / wb;
+  if (!aligned(p->w13, 16) || !aligned(p->w2, 16) || !aligned(p->workspace, 16) || !aligned(p->w13_stride_expert, per16) ||
+      !aligned(p->w13_stride_row, per16) || !aligned(p->w2_stride_expert, per16) || !aligned(p->w2_stride_row, per16))
+    return bad("moe_layer: the workspace and the rows of w13 and w2 must start on 16 bytes");
+  if (!stride_ok(p->x_stride, p->hidden, 1) || !stride_ok(p->out_stride, p->hidden, p->tokens) || !any_stride_ok(p->logits_stride) ||
+      !any_stride_ok(p->w13_stride_expert) || !any_stride_ok(p->w13_stride_row) || !any_stride_ok(p->w2_stride_expert) ||
+      !any_stride_ok(p->w2_stride_row))
+    return bad("moe_layer: a stride is negative, or rows of out overlap");
+  const int64_t pairs = p->tokens * p->topk, slots = pairs < p->experts ? pairs : p->experts;
+  char* ws = (char*)p->workspace;
+  const int64_t plane = pairs * p->inter * 2;
+  MoeArgs a = {(const void*)p->x, (const float*)p->logits, (const void*)p->w13, (const void*)p->w2, (const float*)p->w13_scale, (const float*)p->w2_scale,
+               (void*)p->out, (int32_t*)p->ids, (float*)p->probs, ws, ws + plane, (int32_t*)(ws + 2 * plane),
+               (float*)(ws + 2 * plane + slots * MOE_SLOT * 4), p->x_stride, p->logits_stride, p->out_stride, p->w13_stride_expert,
+               p->w13_stride_row, p->w2_stride_expert, p->w2_stride_row, (int)p->tokens, (int)p->experts, (int)p->topk, (int)p->hidden,
+               (int)p->inter, (int)slots, p->renormalize != 0};
+  return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) {
+    if (int rc = launch(hip, k.fn[kMoeUp + v], (unsigned)(p->inter / 16), (unsigned)slots, UP_WAVES * 64, 0, stream, &a)) return rc;
+    return launch(hip, k.fn[kMoeDown + v], (unsigned)(p->hidden / 16), 1, DOWN_WAVES * 64, moe_partial_bytes(p->tokens, p->topk), stream, &a);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,305 @@
+// kcg_ops_matmul.h — product of e4m3 operands with a scale for each 128 values of a row of A and each 128 x 128 block of B:
+//   C[m, n] = sum_g sa[m, g] sb[n / 128, g] sum_{k in group g} A[m, k] B[n, k]
+// A 16 x 16 x 128 product (E4m3Dot, or WideDot for float32 results) covers exactly one group of k, so its result is the
+// inner sum; it is scaled and added to the float32 accumulator by one fma per element.  B is the first matrix operand: a lane then holds 4 consecutive n of ONE m,
+// needs one activation scale, and stores 4 neighbours of a row of C.
+#pragma once
+#include "kcg_ops_common.h"
+
+namespace kcg_ops {
+
+// ---------------------------------------------------------------------------------------------
+// Few rows (M <= 16 CT): bound by the bytes of B.  A block owns 16 rows of B; its NW waves split K (wave w takes groups
+// w, w + NW, ...), every byte of B goes from memory straight into the matrix operand, 2 KiB per wave and load pair, and
+// the partial sums meet in LDS, added in wave order (the same result on every run).
+// ---------------------------------------------------------------------------------------------
+template <class TC, int CT, int NW>
+__device__ void skinny_kernel(const MatmulArgs& p, float* red) {
+  typedef typename DotOf<TC>::type Dot;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const uint8_t* b = p.b + (int64_t)min(n0 + r, p.N - 1) * p.ldb;      // (rows beyond N: computed from a row that exists, not stored)
+  const float* sb = p.sb + (int64_t)(n0 / GROUP) * p.sb_n;
+  const uint8_t* a[CT];
+  const float* sa[CT];
+#pragma unroll
+  for (int t = 0; t < CT; ++t) {
+    const int64_t m = min(t * 16 + r, p.M - 1);
+    a[t] = p.a + m * p.lda;
+    sa[t] = p.sa + m * p.sa_m;
+  }
+  f32x4 acc[CT];
+#pragma unroll
+  for (int t = 0; t < CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto step = [&](const i32x8& bq, const i32x8 (&aq)[CT], const float (&s)[CT], float sbv) {
+    const typename Dot::frag bf = Dot::make(bq);
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      const f32x4 d = Dot::mma(bf, Dot::make(aq[t]));
+      const float f = s[t] * sbv;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(d[i], f, acc[t][i]);
+    }
+  };
+  const int full = p.K / GROUP;
+  int kb = wave;
+  // U groups at a time, all their loads in front of the first product
+  constexpr int U = CT == 1 ? 4 : 2;
+  for (; kb + (U - 1) * NW < full; kb += U * NW) {
+    i32x8 bq[U], aq[U][CT];
+    float s[U][CT], sbv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (kb + u * NW) * GROUP + g * 32;
+      bq[u] = join(__builtin_nontemporal_load((const u32x4_a*)(b + k)), __builtin_nontemporal_load((const u32x4_a*)(b + k + 16)));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (kb + u * NW) * GROUP + g * 32;
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        aq[u][t] = join(*(const u32x4_a*)(a[t] + k), *(const u32x4_a*)(a[t] + k + 16));
+        s[u][t] = sa[t][(kb + u * NW) * p.sa_k];
+      }
+      sbv[u] = sb[(kb + u * NW) * p.sb_k];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) step(bq[u], aq[u], s[u], sbv[u]);
+  }
+  for (; kb < p.KB; kb += NW) {                    // the rest, the partial last group among it
+    const int k = kb * GROUP + g * 32;
+    const i32x8 bq = join(load16_masked(b, k, p.K), load16_masked(b, k + 16, p.K));
+    i32x8 aq[CT];
+    float s[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      aq[t] = join(load16_masked(a[t], k, p.K), load16_masked(a[t], k + 16, p.K));
+      s[t] = sa[t][kb * p.sa_k];
+    }
+    step(bq, aq, s, sb[kb * p.sb_k]);
+  }
+  // red[wave][t][lane] of 4 floats
+  f32x4* red4 = (f32x4*)red;
+#pragma unroll
+  for (int t = 0; t < CT; ++t) red4[(wave * CT + t) * 64 + lane] = acc[t];
+  __syncthreads();
+  for (int i = threadIdx.x; i < CT * 64; i += NW * 64) {
+    f32x4 v = red4[i];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) v += red4[w * CT * 64 + i];
+    const int m = (i >> 6) * 16 + (i & 15), n = n0 + ((i >> 4) & 3) * 4;
+    if (m < p.M && n < p.N) store4((TC*)p.c + (int64_t)m * p.ldc + n, v, p.N - n, p.c_wide);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Tiles of BM x BN, WM x WN waves, K in steps of one group (128 bytes of a row).
+// LDS: two stages of BM + BN rows of 128 bytes, filled by global_load_lds (16 bytes a lane, no registers).  The chunk at
+// place c of row r is chunk c ^ (r & 7) of that row: 8 lanes that read one chunk column of 8 rows touch all banks.
+// A wave keeps its activation fragments (MB x 16 columns) for a K step and streams the weight fragments (NB x 16 rows)
+// past them, one ahead.  The step of stage s ends (barrier, fetch of the stage after the next into s) in front of the last
+// weight row, whose fragments are in registers by then: the fetch has a whole step to land, the fragment reads of the
+// next step run under the last row's matrix instructions, and the fma of a row run under those of the row behind it.
+// ---------------------------------------------------------------------------------------------
+template <class TC, int BM, int BN, int WM, int WN>
+struct TilePlan {
+  static constexpr int NT = WM * WN * 64;
+  static constexpr int MB = BM / WM / 16, NB = BN / WN / 16;
+  static constexpr int ROWS = BM + BN, STAGE = ROWS * GROUP;
+  static constexpr int FETCH = ROWS * 8 / NT;      // 16-byte chunks a thread fetches for a stage
+  static constexpr int RPF = NT / 8;               // rows one fetch of all threads covers
+  static constexpr int LDS = 2 * STAGE;
+  static_assert(BM % RPF == 0 && BN % RPF == 0 && NB >= 2, "tile plan");
+};
+
+// 16 bytes a lane from base + off into 1 KiB of LDS from lds on.  In assembly, because the compiler would wait for every
+// such fetch in front of each later LDS read; the waits that are needed are written out in the kernel.  (No output
+// registers; vmcnt counts it, which makes the compiler's own waits stricter, never weaker.)
+__device__ __forceinline__ void fetch_lds(const uint8_t* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+
+template <class TC, int BM, int BN, int WM, int WN>
+__device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
+  typedef TilePlan<TC, BM, BN, WM, WN> P;
+  typedef typename DotOf<TC>::type Dot;
+  constexpr int MB = P::MB, NB = P::NB;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  const int r = lane & 15, g = lane >> 4;
+
+  // block -> tile: ids are dealt round-robin to the 8 XCDs; each gets one contiguous part of the order, which walks the
+  // n tiles of 4 tile rows together, so that an XCD's resident tiles share panels of both operands in its L2
+  int bid = blockIdx.x;
+  const int total = p.grid_m * p.grid_n;
+  {
+    const int per = total >> 3, left = total & 7, xcd = bid & 7;
+    bid = xcd * per + min(xcd, left) + (bid >> 3);
+  }
+  constexpr int GM = 4;
+  const int gsize = GM * p.grid_n, grp = bid / gsize, in = bid - grp * gsize;
+  const int gm = min(GM, p.grid_m - grp * GM);
+  const int tm = grp * GM + in % gm, tn = in / gm;
+  const int m0 = tm * BM, n0 = tn * BN;
+
+  // fetch: thread -> row tid / 8 (+ RPF per further fetch), place tid % 8
+  const int frow = tid >> 3, fchunk = (tid & 7) ^ (frow & 7);     // (RPF is a multiple of 8: the swizzle is the same in every fetch)
+  const uint8_t* abase = p.a + (int64_t)m0 * p.lda;
+  const uint8_t* bbase = p.b + (int64_t)n0 * p.ldb;
+  constexpr int FA = BM / P::RPF, FB = BN / P::RPF;
+  unsigned off[FA + FB];
+#pragma unroll
+  for (int f = 0; f < FA; ++f) off[f] = (unsigned)(min(frow + f * P::RPF, p.M - 1 - m0) * (unsigned)p.lda) + fchunk * 16;
+#pragma unroll
+  for (int f = 0; f < FB; ++f) off[FA + f] = (unsigned)(min(frow + f * P::RPF, p.N - 1 - n0) * (unsigned)p.ldb) + fchunk * 16;
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  const unsigned lds_wave = lds0 + wave * 1024;
+  const int KB = p.KB;
+  // a chunk of the partial last group that lies behind K: the row's first chunk of that group instead (cleared in LDS later)
+  const bool ragged = (p.K & (GROUP - 1)) != 0;
+  const bool behind = ragged && fchunk * 16 >= (p.K & (GROUP - 1));
+  auto fetch = [&](int kb) {
+    const unsigned back = behind && kb == KB - 1 ? fchunk * 16 : 0;
+    const unsigned to = lds_wave + (kb & 1) * P::STAGE;
+    const uint8_t* ak = abase + (int64_t)kb * GROUP;
+    const uint8_t* bk = bbase + (int64_t)kb * GROUP;
+#pragma unroll
+    for (int f = 0; f < FA; ++f) fetch_lds(ak, off[f] - back, to + f * P::RPF * GROUP);
+#pragma unroll
+    for (int f = 0; f < FB; ++f) fetch_lds(bk, off[FA + f] - back, to + (BM + f * P::RPF) * GROUP);
+  };
+  // zeros behind K in the stage of the partial last group
+  auto clear_tail = [&](int kb) {
+    const int kt = p.K & (GROUP - 1);
+    uint8_t* st = smem + (kb & 1) * P::STAGE;
+    for (int i = tid; i < P::ROWS * 8; i += P::NT) {
+      const int row = i >> 3, c = i & 7;
+      u32x4_a* at = (u32x4_a*)(st + row * GROUP + ((c ^ (row & 7)) << 4));
+      const int n = kt - c * 16;
+      if (n < 16) {
+        u32x4 v = *at;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int left = n - 4 * w;
+          v[w] = left >= 4 ? v[w] : left <= 0 ? 0u : v[w] & (0xffffffffu >> (32 - 8 * left));
+        }
+        *at = v;
+      }
+    }
+  };
+  // lane's two chunks of a row: g and g + 4 (as good a split of the 128 k values as any, and free of bank conflicts)
+  const unsigned sw0 = ((g ^ (r & 7)) << 4), sw1 = (((g + 4) ^ (r & 7)) << 4);
+  const uint8_t* arow = smem + (wm * MB * 16 + r) * GROUP;
+  const uint8_t* brow = smem + (BM + wn * NB * 16 + r) * GROUP;
+  auto frag = [&](const uint8_t* base, int i, int stage) {
+    const uint8_t* q = base + stage * P::STAGE + i * 16 * GROUP;
+    return join(*(const u32x4_a*)(q + sw0), *(const u32x4_a*)(q + sw1));
+  };
+  // scales: one of the activations per lane and column tile, one of the weights per 128 of the wave's rows of B
+  constexpr int SPAN = NB * 16;
+  constexpr int SB = SPAN >= GROUP ? SPAN / GROUP : 1;
+  const int nb0 = (n0 + wn * SPAN) / GROUP, nb_last = (p.N - 1) / GROUP;
+  unsigned sa_off[MB];
+#pragma unroll
+  for (int j = 0; j < MB; ++j) sa_off[j] = (unsigned)min((wm * MB + j) * 16 + r, p.M - 1 - m0) * (unsigned)p.sa_m;
+  const float* sa_tile = p.sa + (int64_t)m0 * p.sa_m;
+  float sa_raw[MB], sb_raw[SB];
+  auto load_scales = [&](int kb) {
+#pragma unroll
+    for (int q = 0; q < SB; ++q) sb_raw[q] = p.sb[(int64_t)min(nb0 + q, nb_last) * p.sb_n + (int64_t)kb * p.sb_k];
+    const float* base = sa_tile + (int64_t)kb * p.sa_k;
+#pragma unroll
+    for (int j = 0; j < MB; ++j) sa_raw[j] = base[sa_off[j]];
+  };
+  float s[SB][MB];
+  auto join_scales = [&]() {
+#pragma unroll
+    for (int q = 0; q < SB; ++q)
+#pragma unroll
+      for (int j = 0; j < MB; ++j) s[q][j] = sa_raw[j] * sb_raw[q];
+  };
+
+  f32x4 acc[NB][MB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (KB > 0) {
+    load_scales(0);
+    fetch(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    join_scales();
+    if (ragged && KB == 1) {
+      clear_tail(0);
+      __syncthreads();
+    }
+    if (KB > 1) fetch(1);
+    i32x8 am[MB], bn[2];
+#pragma unroll
+    for (int j = 0; j < MB; ++j) am[j] = frag(arow, j, 0);
+    bn[0] = frag(brow, 0, 0);
+    // Products q = i MB + j run through d[q % 3]; the fma of a product follows the second product behind it, when its result is
+    // there without a wait.
+    f32x4 d[3];
+    auto add = [&](auto q_c) {
+      constexpr int q = decltype(q_c)::value, i = q / MB, j = q % MB;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[q % 3][e], s[i * 16 / GROUP][j], acc[i][j][e]);
+      // (here, not behind the branches at the end of the step, where the compiler would gather them and keep every d until then)
+      asm volatile("" : "+v"(acc[i][j]));
+    };
+
+    for (int kb = 0; kb < KB; ++kb) {
+      const int stage = kb & 1;
+      const int nx = min(kb + 1, KB - 1);
+      typename Dot::frag af[MB];
+#pragma unroll
+      for (int j = 0; j < MB; ++j) af[j] = Dot::make(am[j]);
+      load_scales(nx);                            // (used a step later: the loads have the whole step)
+      static_for<0, NB>([&](auto i_c) {
+        constexpr int i = decltype(i_c)::value;
+        if constexpr (i == NB - 1) {
+          // every fragment of this stage is in registers or on its way; the next stage has had a step to land
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          if (ragged && kb + 1 == KB - 1) {
+            clear_tail(kb + 1);
+            __syncthreads();
+          }
+          if (kb + 2 < KB) fetch(kb + 2);
+        }
+        if constexpr (i + 1 < NB) bn[(i + 1) & 1] = frag(brow, i + 1, stage);
+        const typename Dot::frag bf = Dot::make(bn[i & 1]);
+        static_for<0, MB>([&](auto j_c) {
+          constexpr int j = decltype(j_c)::value, q = i * MB + j;
+          d[q % 3] = Dot::mma(bf, af[j]);
+          if constexpr (i == NB - 1) am[j] = frag(arow, j, nx & 1);      // (after the last step: the same stage again, unused)
+          if constexpr (q >= 2) add(Int<q - 2>());
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      bn[0] = frag(brow, 0, nx & 1);
+      add(Int<NB * MB - 2>());
+      add(Int<NB * MB - 1>());
+      join_scales();
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < MB; ++j) {
+    const int m = m0 + (wm * MB + j) * 16 + r;
+    if (m < p.M) {
+      TC* c = (TC*)p.c + (int64_t)m * p.ldc;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int n = n0 + wn * SPAN + i * 16 + g * 4;
+        if (n < p.N) store4(c + n, acc[i][j], p.N - n, p.c_wide);
+      }
+    }
+  }
+}
+
+}  // namespace kcg_ops

@@ -1,0 +1,459 @@
+"""The operators of the 8-bit path on the GPU against their definitions in 64 bits (tests/ops_reference.py holds the bounds)."""
+import pytest
+import torch
+
+from codegendemo_amd import _native, _native_ops
+from codegendemo_amd.kcg.Operators.matmul_fp8 import matmul_fp8
+from codegendemo_amd.kcg.Operators.moe import moe_layer
+from codegendemo_amd.kcg.Operators.quant import rmsnorm_quant, swiglu_quant
+from tests import ops_reference as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+E4M3 = torch.float8_e4m3fn
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+FLOOR_SCALE = torch.tensor(1e-10) / torch.tensor(448.0)      # one float32 quotient, rounded once (on a GPU torch multiplies by 1 / 448)
+
+
+def gen(seed=1):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def rows8(rows, cols, fill=0x55, extra=0):
+    """An e4m3 matrix with padded rows, its bytes preset; rows `extra` apart beyond what they need."""
+    base = torch.full((rows, R.groups(cols) * 128 + extra), fill, dtype=torch.uint8, device=DEV)
+    return base, base.view(E4M3)[:, :cols]
+
+
+def to8(v, block_rows, fill=0x7f):
+    """Values in e4m3 with scales; what lies behind the rows' ends are NaN bytes."""
+    r, c = v.shape
+    p = torch.zeros(-(-r // block_rows) * block_rows, R.groups(c) * 128, device=DEV)
+    p[:r, :c] = v
+    p = p.view(-1, block_rows, R.groups(c), 128)
+    s = p.abs().amax((1, 3)).clamp_min(1e-10) / 448
+    base, q = rows8(r, c, fill)
+    q.copy_((p / s[:, None, :, None]).reshape(-1, R.groups(c) * 128)[:r, :c].to(E4M3))
+    return q, s.contiguous()
+
+
+# ---- norm --------------------------------------------------------------------------------------------------------------------
+
+NORMS = [(1, 1, BF16), (1, 16, F16), (3, 127, F32), (2, 128, BF16), (5, 129, BF16), (7, 512, F16), (4, 513, BF16), (9, 1000, F16), (3, 2048, F32), (2, 2056, BF16),
+         (2, 4097, BF16), (3, 8192, BF16), (2, 8200, F32), (2, 16384, BF16), (2, 16385, F16), (1, 40007, BF16)]
+
+
+@pytest.mark.parametrize("t,h,dtype", NORMS)
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm(t, h, dtype, residual):
+    print(f"[case] norm {t}x{h} {dtype} residual={residual}", flush=True)
+    g = gen(h)
+    x = (torch.randn(t, h + 3, device=DEV, generator=g) * 3).to(dtype)[:, :h]              # rows that start anywhere
+    res = torch.randn(t, h, device=DEV, generator=g).to(dtype) if residual else None
+    weight = torch.randn(h, device=DEV, generator=g).to(F32 if h % 2 else dtype)
+    base, q = rows8(t, h, extra=16)
+    q, scale, y, r_out = rmsnorm_quant(x, weight, 1e-5, res, q=q, want_y=True)
+    r, want = R.norm64(x, res, weight, 1e-5)
+    if residual:
+        assert bool(((r_out.double() - r).abs() <= r.abs() * (R.half_step(dtype) + R.U) + R.smallest(dtype)).all())
+    else:
+        assert r_out is None
+    assert y.dtype is dtype
+    assert bool(((y.double() - want).abs() <= want.abs() * (R.half_step(dtype) + R.NORM_REL) + R.smallest(dtype)).all())
+    R.check_quantized(q, scale, want, R.NORM_REL)
+    assert bool((base[:, h:] == 0x55).all()), "bytes behind the rows' ends were written"
+
+
+def test_norm_leaves_other_rows_and_columns_alone():
+    g = gen()
+    big = torch.full((6, 300), 7.0, dtype=BF16, device=DEV)
+    scales = torch.full((6, 5), -1.0, device=DEV)
+    base, q = rows8(6, 200)
+    x = torch.randn(3, 200, device=DEV, generator=g).to(BF16)
+    rmsnorm_quant(x, torch.ones(200, dtype=BF16, device=DEV), 1e-6, x, residual_out=big[1:4, 8:208], q=q[1:4], scale=scales[1:4, 2:4], y=big[1:4, 8:208])
+    torch.cuda.synchronize()
+    assert bool((big[0] == 7).all()) and bool((big[4:] == 7).all()) and bool((big[:, :8] == 7).all()) and bool((big[:, 208:] == 7).all())
+    assert bool((scales[:, :2] == -1).all()) and bool((scales[:, 4:] == -1).all()) and bool((scales[0] == -1).all()) and bool((scales[4:] == -1).all())
+    assert bool((base[0] == 0x55).all()) and bool((base[4:] == 0x55).all()) and bool((scales[1:4, 2:4] > 0).all())
+
+
+@pytest.mark.parametrize("h", [300, 9000, 20000])
+def test_norm_in_place_and_transposed_scales(h):
+    """residual_out may be the residual; scales of any strides."""
+    g = gen(h)
+    x, res = (torch.randn(4, h, device=DEV, generator=g).to(BF16) for _ in range(2))
+    w = torch.ones(h, dtype=BF16, device=DEV)
+    q0, s0, _, r0 = rmsnorm_quant(x, w, 1e-6, res)
+    mine = res.clone()
+    st = torch.empty(R.groups(h), 4, device=DEV).t()
+    q1, s1, y, r1 = rmsnorm_quant(x, w, 1e-6, mine, residual_out=mine, scale=st)
+    assert r1 is mine and y is None and s1.data_ptr() == st.data_ptr()
+    assert torch.equal(r0, mine) and torch.equal(s0, s1) and torch.equal(q0.float(), q1.float())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_of_rows_that_are_not_ordinary(dtype):
+    """Zeros, the type's largest values, NaN and infinity in one row each: the others do not notice."""
+    g = gen()
+    h = 400
+    x = torch.randn(6, h, device=DEV, generator=g).to(dtype)
+    clean = x.clone()
+    x[0] = 0
+    x[1] = 1e18
+    x[2, 5] = float("nan")
+    x[3, 200] = float("inf")
+    x[4] = 1e-30
+    w = torch.ones(h, dtype=dtype, device=DEV)
+    q, s, y, _ = rmsnorm_quant(x, w, 1e-6, want_y=True)
+    qc, sc, yc, _ = rmsnorm_quant(clean, w, 1e-6, want_y=True)
+    assert bool((q[0].float() == 0).all()) and bool((s[0].cpu() == FLOOR_SCALE).all()) and bool((y[0] == 0).all())
+    R.check_quantized(q[1:2], s[1:2], R.norm64(x, None, w, 1e-6)[1][1:2], R.NORM_REL)
+    assert bool(torch.isnan(s[2]).all()) and bool(torch.isnan(q[2].float()).all()) and bool(torch.isnan(y[2]).all())
+    assert bool(torch.isnan(y[3, 200])) and bool(torch.isnan(s[3, 1])) and bool((y[3, :200] == 0).all()) and bool((q[3, :128].float() == 0).all())
+    R.check_quantized(q[4:5], s[4:5], R.norm64(x, None, w, 1e-6)[1][4:5], R.NORM_REL)
+    assert torch.equal(q[5].float(), qc[5].float()) and torch.equal(s[5], sc[5]) and torch.equal(y[5], yc[5])
+
+
+# ---- activation --------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("t,i,dtype", [(1, 1, BF16), (3, 16, F16), (2, 127, F32), (5, 128, BF16), (33, 200, F16), (4, 1001, BF16), (70, 4096, BF16), (3, 11008, F32)])
+def test_swiglu(t, i, dtype):
+    print(f"[case] swiglu {t}x{i} {dtype}", flush=True)
+    g = gen(i)
+    gate_up = (torch.randn(t, 2 * i + 5, device=DEV, generator=g) * 4).to(dtype)[:, :2 * i]
+    base, q = rows8(t, i, extra=32)
+    q, scale = swiglu_quant(gate_up, q=q)
+    R.check_quantized(q, scale, R.swiglu64(gate_up), R.SWIGLU_REL)
+    assert bool((base[:, i:] == 0x55).all())
+
+
+def test_swiglu_of_large_gates():
+    """exp(-gate) that overflows gives 0, not NaN; NaN stays in its group."""
+    gate = torch.tensor([-200.0, -100.0, -88.0, 0.0, 88.0, 200.0], device=DEV)
+    x = torch.zeros(2, 512, device=DEV)
+    x[0, :6], x[0, 256:262] = gate, 1.0
+    x[1, 130], x[1, 256:] = float("nan"), 1.0
+    q, s = swiglu_quant(x)
+    R.check_quantized(q[:1], s[:1], R.swiglu64(x[:1]), R.SWIGLU_REL)
+    assert bool(torch.isfinite(q[0].float()).all()) and bool(torch.isnan(s[1, 1])) and bool((s[1, :1] > 0).all()) and bool((q[1, :128].float() == 0).all())
+
+
+# ---- product -----------------------------------------------------------------------------------------------------------------
+
+MATMULS = [(1, 1, 1, F32), (1, 16, 128, BF16), (2, 5, 15, F32), (3, 100, 127, F16), (15, 129, 129, F32), (16, 300, 1000, BF16), (17, 64, 256, F32), (32, 4096, 200, F16),
+           (33, 200, 2300, F32), (64, 1000, 520, BF16), (65, 64, 128, F32), (100, 70, 100, F16), (128, 128, 384, F32), (129, 257, 1000, F32), (200, 999, 130, BF16),
+           (1, 512, 16384, F32), (256, 256, 4096, F32), (2100, 1500, 300, F32), (1800, 1790, 129, BF16), (3500, 3700, 200, F32), (4096, 4000, 640, F16), (3601, 3585, 127, BF16)]
+
+
+@pytest.mark.parametrize("m,n,k,out", MATMULS)
+def test_matmul(m, n, k, out):
+    print(f"[case] matmul {m}x{n}x{k} {out}", flush=True)
+    g = gen(m + n + k)
+    a, sa = to8(torch.randn(m, k, device=DEV, generator=g) * torch.exp(torch.randn(m, 1, device=DEV, generator=g)), 1)
+    b, sb = to8(torch.randn(n, k, device=DEV, generator=g) * torch.exp(torch.randn(n, 1, device=DEV, generator=g)), 128)
+    big = torch.full((m + 2, n + 9), 5.0, dtype=out, device=DEV)
+    c = matmul_fp8(a, sa, b, sb, out=big[1:m + 1, 4:n + 4])
+    R.check_matmul(c, a, sa, b, sb)
+    big[1:m + 1, 4:n + 4] = 5.0
+    assert bool((big == 5).all()), "something outside the output was written"
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 48, 1024), (37, 80, 640), (130, 140, 1152), (2048, 1536, 640), (4096, 3600, 256)])
+def test_matmul_of_whole_numbers_is_exact(m, n, k):
+    """Small whole numbers and powers of two as scales: every partial sum is a whole number below 2^24 in units of the
+    smallest scale product, so float32 has to hold it exactly, whatever the order."""
+    g = gen(k)
+    a = torch.randint(-3, 4, (m, k), device=DEV, generator=g).float().to(E4M3)
+    b = torch.randint(-3, 4, (n, k), device=DEV, generator=g).float().to(E4M3)
+    sa = 2.0 ** torch.randint(-1, 2, (m, k // 128), device=DEV, generator=g).float()
+    sb = 2.0 ** torch.randint(-1, 2, (R.groups(n), k // 128), device=DEV, generator=g).float()
+    want = R.widen(a, sa, False) @ R.widen(b, sb, True).t().contiguous()
+    assert 4 * 9 * 16 * k < 2 ** 24
+    assert torch.equal(matmul_fp8(a, sa, b, sb, out_dtype=F32).double(), want)
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_matmul_strides_and_orders(m):
+    """Scales of other strides, rows further apart than they are long, a single row of a column-major view."""
+    g = gen(m)
+    n, k = 272, 400
+    a, sa = to8(torch.randn(m, k, device=DEV, generator=g), 1)
+    b, sb = to8(torch.randn(n, k, device=DEV, generator=g), 128)
+    want = matmul_fp8(a, sa, b, sb, out_dtype=F32)
+    wide = torch.zeros(m, 1024, dtype=torch.uint8, device=DEV).view(E4M3)[:, 512:512 + k]
+    wide.copy_(a)
+    got = matmul_fp8(wide, sa.t().contiguous().t(), b, sb.t().contiguous().t(), out_dtype=F32)
+    assert torch.equal(got, want)
+    one = matmul_fp8(a, sa[:, :1].expand(m, R.groups(k)), b, sb[:1, :1].expand(R.groups(n), R.groups(k)), out_dtype=F32)   # strides of 0
+    R.check_matmul(one, a, sa[:, :1].expand(m, R.groups(k)), b, sb[:1, :1].expand(R.groups(n), R.groups(k)))
+
+
+@pytest.mark.parametrize("m,n", [(20, 100), (200, 300), (3600, 3600)])
+def test_matmul_keeps_nan_in_its_row(m, n):
+    g = gen(m)
+    k = 300
+    a, sa = to8(torch.randn(m, k, device=DEV, generator=g), 1)
+    b, sb = to8(torch.randn(n, k, device=DEV, generator=g), 128)
+    clean = matmul_fp8(a, sa, b, sb)
+    a.view(torch.uint8)[m // 2, k - 1] = 0x7f
+    sa[m - 1, 1] = float("inf")
+    got = matmul_fp8(a, sa, b, sb)
+    assert bool(torch.isnan(got[m // 2]).all()) and not bool(torch.isfinite(got[m - 1]).any())
+    keep = torch.ones(m, dtype=torch.bool)
+    keep[m // 2] = keep[m - 1] = False
+    assert torch.equal(got[keep], clean[keep])
+
+
+def test_matmul_without_k_is_zero():
+    for m in (3, 100):
+        a, b = torch.empty(m, 0, dtype=E4M3, device=DEV), torch.empty(40, 0, dtype=E4M3, device=DEV)
+        c = torch.full((m, 40), 3.0, device=DEV)
+        matmul_fp8(a, torch.empty(m, 0, device=DEV), b, torch.empty(1, 0, device=DEV), out=c)
+        assert bool((c == 0).all())
+
+
+def test_matmul_beyond_32_bits():
+    """Rows of a and of c whose byte offsets pass 2^32."""
+    print("[case] matmul far rows", flush=True)
+    m, n, k = 1100, 64, 128
+    far = torch.empty(m, 1 << 22, dtype=torch.uint8, device=DEV).view(E4M3)[:, :k]         # 4.6 GB
+    g = gen()
+    a, sa = to8(torch.randn(m, k, device=DEV, generator=g), 1)
+    b, sb = to8(torch.randn(n, k, device=DEV, generator=g), 128)
+    far.copy_(a)
+    out = torch.empty(m, 1 << 20, dtype=F32, device=DEV)[:, :n]
+    matmul_fp8(far, sa, b, sb, out=out)
+    assert torch.equal(out, matmul_fp8(a, sa, b, sb, out_dtype=F32))
+
+
+# ---- experts -----------------------------------------------------------------------------------------------------------------
+
+def experts(g, e, h, i, weights):
+    w13, w2 = torch.randn(e, 2 * i, h, device=DEV, generator=g) * h ** -0.5, torch.randn(e, h, i, device=DEV, generator=g) * i ** -0.5
+    if weights is BF16:
+        return w13.to(BF16), w2.to(BF16), None, None
+    out = []
+    for w in (w13, w2):
+        qs = [to8(v, 128) for v in w]
+        out.append((torch.stack([q for q, _ in qs]).contiguous(), torch.stack([s for _, s in qs])))
+    return out[0][0], out[1][0], out[0][1], out[1][1]
+
+
+MOES = [(1, 1, 1, 16, 16, E4M3, BF16), (1, 64, 8, 256, 128, E4M3, BF16), (1, 4, 2, 144, 80, E4M3, F16), (3, 8, 2, 1040, 208, BF16, BF16), (16, 4, 4, 272, 144, E4M3, BF16),
+        (17, 8, 3, 256, 400, E4M3, F16), (33, 3, 2, 128, 272, BF16, BF16), (64, 2, 1, 512, 128, E4M3, BF16), (64, 64, 16, 256, 64, E4M3, BF16), (5, 512, 10, 128, 48, E4M3, BF16),
+        (64, 130, 8, 144, 112, E4M3, F16), (2, 300, 16, 64, 32, BF16, BF16), (64, 1, 1, 128, 2064, E4M3, BF16)]
+
+
+@pytest.mark.parametrize("t,e,k,h,i,weights,dtype", MOES)
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_moe(t, e, k, h, i, weights, dtype, renormalize):
+    print(f"[case] moe T={t} E={e} k={k} H={h} I={i} {weights} {dtype} renormalize={renormalize}", flush=True)
+    g = gen(t + e + h)
+    w13, w2, s13, s2 = experts(g, e, h, i, weights)
+    x = torch.randn(t, h + 8, device=DEV, generator=g).to(dtype)[:, :h]
+    logits = (torch.randn(t, e, device=DEV, generator=g) * 2).to(BF16).float()              # equal ones among many experts
+    big = torch.full((t + 2, h + 16), 9.0, dtype=dtype, device=DEV)
+    out, ids, probs = moe_layer(x, logits, k, w13, w2, s13, s2, renormalize, out=big[1:t + 1, 8:h + 8])
+    want, err, want_ids, want_probs = R.moe64(x, logits, k, w13, w2, s13, s2, renormalize)
+    assert torch.equal(ids.long(), want_ids)
+    # exp to 2 ulp, E terms, a quotient; the exponent's argument is a difference of bf16 numbers below 16: half a step of that
+    assert bool(((probs.double() - want_probs).abs() <= want_probs * (2 * 4 + e + 2 + 2 * 16) * R.U).all())
+    off = (out.double() - want).abs()
+    allowed = want.abs() * R.half_step(dtype) + err + want.abs() * (e + 42) * R.U + R.smallest(dtype)
+    # (p's own error reaches every term of the sum, which may cancel: err is proportional to the magnitudes, not to the sum)
+    allowed = allowed + err * (e + 42) / 32
+    assert bool((off <= allowed).all()), f"off by up to {(off / allowed).max().item()} of what is allowed"
+    big[1:t + 1, 8:h + 8] = 9.0
+    assert bool((big == 9).all()), "something outside the output was written"
+
+
+def test_moe_masked_logits_ties_and_nan():
+    """-inf takes experts out, down to none; equal logits choose the lower expert; NaN and infinity of a token or of an
+    expert that a token does not weigh stay where they are."""
+    g = gen(3)
+    t, e, k, h, i = 6, 8, 3, 128, 64
+    w13, w2, s13, s2 = experts(g, e, h, i, E4M3)
+    s2[7] = float("inf")                                     # an expert whose every output is infinite or NaN
+    x = torch.randn(t, h, device=DEV, generator=g).to(BF16)
+    logits = torch.randn(t, e, device=DEV, generator=g)
+    logits[:, 7] = float("-inf")
+    logits[1] = float("-inf")                                # nothing left
+    logits[2] = float("-inf")
+    logits[2, 5] = 0.25                                      # one left of three
+    logits[3] = 1.0
+    logits[3, 7] = float("-inf")
+    logits[3, 0] = -0.0                                      # equal ones: 1, 2, 3
+    logits[4, 2] = float("nan")
+    for renormalize in (True, False):
+        out, ids, probs = moe_layer(x, logits, k, w13, w2, s13, s2, renormalize)
+        for row in ids.tolist():
+            assert len(set(row)) == k and all(0 <= v < e for v in row)
+        assert bool((out[1] == 0).all()) and bool((probs[1] == 0).all())
+        assert ids[2, 0].item() == 5 and probs[2].tolist() == [1.0, 0.0, 0.0]
+        assert ids[3].tolist() == [1, 2, 3]
+        assert bool(torch.isnan(out[4]).all()) and ids[4, 0].item() == 2
+        for row in (0, 2, 3, 5):
+            want, err, _, _ = R.moe64(x[row:row + 1], logits[row:row + 1], k, w13, w2, s13, s2, renormalize)
+            assert bool(((out[row:row + 1].double() - want).abs() <= want.abs() * (R.half_step(BF16) + 64 * R.U) + err * 3 + R.smallest(BF16)).all()), row
+
+
+def test_moe_of_a_fully_repeated_choice():
+    """All tokens choose the same experts: columns beyond 16, 32 and 48 of one expert."""
+    g = gen(5)
+    t, e, k, h, i = 64, 6, 2, 256, 128
+    w13, w2, s13, s2 = experts(g, e, h, i, E4M3)
+    x = torch.randn(t, h, device=DEV, generator=g).to(BF16)
+    logits = torch.randn(1, e, device=DEV, generator=g).expand(t, e)                    # a row stride of 0
+    out, ids, probs = moe_layer(x, logits, k, w13, w2, s13, s2)
+    want, err, want_ids, _ = R.moe64(x, logits, k, w13, w2, s13, s2, True)
+    assert torch.equal(ids.long(), want_ids)
+    assert bool(((out.double() - want).abs() <= want.abs() * (R.half_step(BF16) + 64 * R.U) + err * 3 + R.smallest(BF16)).all())
+
+
+# ---- the set as it is used -----------------------------------------------------------------------------------------------------
+
+def block(x, residual, norm_w, wgu, sgu, wd, sd, out=None):
+    q, s, _, r = rmsnorm_quant(x, norm_w, 1e-6, residual)
+    hq, hs = swiglu_quant(matmul_fp8(q, s, wgu, sgu))
+    return matmul_fp8(hq, hs, wd, sd, out=out), r
+
+
+@pytest.mark.parametrize("t", [1, 19, 150])
+def test_a_dense_block_of_them(t):
+    """norm -> product -> activation -> product, each stage against the definition on what the stage before it gave."""
+    g = gen(t)
+    h, i = 1000, 1304
+    x, res = (torch.randn(t, h, device=DEV, generator=g).to(BF16) for _ in range(2))
+    norm_w = torch.rand(h, device=DEV, generator=g).to(BF16)
+    wgu, sgu = to8(torch.randn(2 * i, h, device=DEV, generator=g) * h ** -0.5, 128)
+    wd, sd = to8(torch.randn(h, i, device=DEV, generator=g) * i ** -0.5, 128)
+    q, s, _, r = rmsnorm_quant(x, norm_w, 1e-6, res)
+    R.check_quantized(q, s, R.norm64(x, res, norm_w, 1e-6)[1], R.NORM_REL)
+    gu = matmul_fp8(q, s, wgu, sgu)
+    R.check_matmul(gu, q, s, wgu, sgu)
+    hq, hs = swiglu_quant(gu)
+    R.check_quantized(hq, hs, R.swiglu64(gu), R.SWIGLU_REL)
+    R.check_matmul(matmul_fp8(hq, hs, wd, sd), hq, hs, wd, sd)
+    # on a side stream, nothing waited for in between: the same bits
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again, r2 = block(x, res, norm_w, wgu, sgu, wd, sd)
+    side.synchronize()
+    assert torch.equal(again, matmul_fp8(hq, hs, wd, sd)) and torch.equal(r2, r)
+
+
+def test_a_routed_block_captured_and_replayed():
+    """norm (16 and 8-bit rows) -> router -> experts, and the dense block, in one graph: every replay equals the eager result on
+    the inputs of the moment, with eager work in between; a second graph of the same calls does not disturb the first."""
+    g = gen(9)
+    t, e, k, h, i = 8, 16, 4, 512, 256
+    w13, w2, s13, s2 = experts(g, e, h, i, E4M3)
+    router = torch.randn(h, e, device=DEV, generator=g) * h ** -0.5
+    norm_w = torch.rand(h, device=DEV, generator=g).to(BF16)
+    wgu, sgu = to8(torch.randn(2 * i, h, device=DEV, generator=g) * h ** -0.5, 128)
+    wd, sd = to8(torch.randn(h, i, device=DEV, generator=g) * i ** -0.5, 128)
+    x, res = (torch.zeros(t, h, dtype=BF16, device=DEV) for _ in range(2))
+
+    def step():
+        d, r = block(x, res, norm_w, wgu, sgu, wd, sd)
+        _, _, y, r2 = rmsnorm_quant(d, norm_w, 1e-6, r, want_y=True)
+        out, ids, probs = moe_layer(y, y.float() @ router, k, w13, w2, s13, s2)
+        return r2, out, ids, probs
+
+    _native_ops.load(0)
+    step()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step())
+        graphs.append(graph)
+    for rep in range(4):
+        x.copy_(torch.randn(t, h, device=DEV, generator=g))
+        res.copy_(torch.randn(t, h, device=DEV, generator=g))
+        torch.cuda.synchronize()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        torch.cuda.synchronize()
+        for out in outs:
+            for a, b in zip(out, eager):
+                assert torch.equal(a, b), f"replay {rep}"
+
+
+def test_two_runs_give_the_same_bits():
+    g = gen(11)
+    w13, w2, s13, s2 = experts(g, 16, 512, 256, E4M3)
+    x = torch.randn(40, 512, device=DEV, generator=g).to(BF16)
+    logits = torch.randn(40, 16, device=DEV, generator=g)
+    a, sa = to8(torch.randn(50, 4096, device=DEV, generator=g), 1)
+    b, sb = to8(torch.randn(700, 4096, device=DEV, generator=g), 128)
+    first = moe_layer(x, logits, 4, w13, w2, s13, s2)[0], matmul_fp8(a, sa, b, sb)
+    for _ in range(5):
+        assert torch.equal(moe_layer(x, logits, 4, w13, w2, s13, s2)[0], first[0]) and torch.equal(matmul_fp8(a, sa, b, sb), first[1])
+
+
+def test_empty_tensors():
+    q, s, y, r = rmsnorm_quant(torch.empty(0, 64, dtype=BF16, device=DEV), torch.ones(64, dtype=BF16, device=DEV))
+    assert q.shape == (0, 64) and s.shape == (0, 1)
+    assert swiglu_quant(torch.empty(3, 0, dtype=BF16, device=DEV))[0].shape == (3, 0)
+    assert matmul_fp8(q, s, *to8(torch.ones(5, 64, device=DEV), 128)).shape == (0, 5)
+    w13, w2, s13, s2 = experts(gen(), 2, 32, 16, E4M3)
+    assert moe_layer(torch.empty(0, 32, dtype=BF16, device=DEV), torch.empty(0, 2, device=DEV), 1, w13, w2, s13, s2)[0].shape == (0, 32)
+
+
+# ---- refusals that name the argument -------------------------------------------------------------------------------------------
+
+def test_refused_arguments():
+    g = gen()
+    x = torch.randn(4, 256, device=DEV, generator=g).to(BF16)
+    w = torch.ones(256, dtype=BF16, device=DEV)
+    for bad in (dict(weight=w[:255]), dict(weight=w.half()), dict(residual=x[:, :128]), dict(residual=x.float()), dict(residual_out=x), dict(y=x.float()),
+                dict(scale=torch.empty(4, 3, device=DEV)), dict(q=torch.empty(4, 256, dtype=torch.uint8, device=DEV)), dict(residual=x.t().contiguous().t()),
+                dict(weight=w.cpu())):
+        with pytest.raises((TypeError, ValueError)):
+            rmsnorm_quant(**{"x": x, "weight": w, **bad})
+    with pytest.raises(TypeError):
+        rmsnorm_quant(x.double(), w)
+    with pytest.raises(_native.KcgError, match="16 bytes"):
+        rmsnorm_quant(x[:, :250], w[:250], q=torch.empty(4, 250, dtype=E4M3, device=DEV))
+    with pytest.raises(ValueError):
+        swiglu_quant(x[:, :255])
+    a, sa = to8(torch.ones(4, 256, device=DEV), 1)
+    b, sb = to8(torch.ones(300, 256, device=DEV), 128)
+    for bad in ((a, sa, b[:, :128], sb), (a, sa[:, :1], b, sb), (a, sa, b, sb[:2]), (a, sa.double(), b, sb), (x, sa, b, sb), (a, sa, b, sb.cpu()), (a[0], sa, b, sb)):
+        with pytest.raises((TypeError, ValueError)):
+            matmul_fp8(*bad)
+    with pytest.raises(TypeError):
+        matmul_fp8(a, sa, b, sb, out_dtype=torch.float64)
+    with pytest.raises(ValueError):
+        matmul_fp8(a, sa, b, sb, out=torch.empty(4, 301, device=DEV))
+    w13, w2, s13, s2 = experts(g, 4, 256, 64, E4M3)
+    logits = torch.zeros(4, 4, device=DEV)
+    good = dict(x=x, logits=logits, topk=2, w13=w13, w2=w2, w13_scale=s13, w2_scale=s2)
+    moe_layer(**good)
+    for bad in (dict(logits=logits.half()), dict(logits=logits[:3]), dict(w2=w2[:3]), dict(w13=w13[:, :127]), dict(w13_scale=None), dict(w2_scale=s2[:, :, :0]),
+                dict(x=x.float()), dict(w13=w13.to(F16), w2=w2.to(F16)), dict(w13=w13.float().to(BF16), w2=w2.float().to(BF16)), dict(topk=5), dict(topk=0),
+                dict(out=torch.empty(4, 256, device=DEV))):
+        with pytest.raises((TypeError, ValueError, _native.KcgError)):
+            moe_layer(**{**good, **bad})
+    with pytest.raises(_native.KcgError, match="few tokens"):
+        moe_layer(x.repeat(17, 1), logits.repeat(17, 1), 2, w13, w2, s13, s2)
+
+
+@pytest.mark.parametrize("h,dtype", [(40, F32), (1000, BF16), (3000, F32), (20000, BF16)])
+@pytest.mark.parametrize("size", [3e38, 1e20, 1e-25, 1e-38])
+def test_norm_of_rows_whose_squares_leave_the_range(h, dtype, size):
+    g = gen(h)
+    x = ((torch.rand(2, h, device=DEV, generator=g) + 0.1) * 0.9 * size).to(dtype)
+    w = torch.ones(h, dtype=dtype, device=DEV)
+    for eps in (0.0, 1e-6):
+        q, s, y, _ = rmsnorm_quant(x, w, eps, want_y=True)
+        want = R.norm64(x, None, w, eps)[1]
+        assert bool(((y.double() - want).abs() <= want.abs() * (R.half_step(dtype) + R.NORM_REL) + R.smallest(dtype)).all())
+        R.check_quantized(q, s, want, R.NORM_REL)
