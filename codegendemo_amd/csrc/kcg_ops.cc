@@ -24,7 +24,7 @@ using kcg::HostHip;
 using namespace kcg_ops;
 
 // ---- kernels ---------------------------------------------------------------------------------
-enum { kNorm = 0, kSwiglu = kNorm + 21, kSkinny = kSwiglu + 3, kTile = kSkinny + 9, kMoeUp = kTile + 8, kMoeDown = kMoeUp + 3, kNumKernels = kMoeDown + 3 };
+enum { kNorm = 0, kSwiglu = kNorm + 21, kSkinny = kSwiglu + 3, kTile = kSkinny + 24, kMoeUp = kTile + 8, kMoeDown = kMoeUp + 3, kNumKernels = kMoeDown + 6 };
 
 std::string kernel_symbol(int i) {
   static const char* const types[3] = {"bf16", "f16", "f32"};
@@ -33,10 +33,13 @@ std::string kernel_symbol(int i) {
   static const char* const moe[3] = {"e4m3_bf16", "e4m3_f16", "bf16_bf16"};
   if (i < kSwiglu) return std::string("kcg_norm_") + types[i / 7] + "_" + norm[i % 7];
   if (i < kSkinny) return std::string("kcg_swiglu_") + types[i - kSwiglu];
-  if (i < kTile) return std::string("kcg_mm8_skinny_") + types[(i - kSkinny) / 3] + "_" + std::to_string(1 << (i - kSkinny) % 3);
+  if (i < kTile) {
+    const int v = (i - kSkinny) % 8;
+    return std::string("kcg_mm8_skinny_") + types[(i - kSkinny) / 8] + "_" + std::to_string(v / 2 + 1) + "x" + std::to_string(v % 2 + 1);
+  }
   if (i < kMoeUp) return std::string("kcg_mm8_tile_") + tile[i - kTile];
   if (i < kMoeDown) return std::string("kcg_moe_up_") + moe[i - kMoeUp];
-  return std::string("kcg_moe_down_") + moe[i - kMoeDown];
+  return std::string("kcg_moe_down_") + moe[(i - kMoeDown) / 2] + "_" + std::to_string((i - kMoeDown) % 2);
 }
 
 struct DeviceKernels {
@@ -62,7 +65,11 @@ struct OnDevice {
   }
 };
 
-int moe_partial_bytes(int64_t tokens, int64_t topk) { return (int)(tokens * (topk > 16 ? topk : 16) * 16 * 4); }
+// LDS of a block of the experts' second kernel: 16 partial sums for each pair and part of I, of which there are tokens * 16
+// at most (parts = 16 / items, and items >= topk <= 16); one form keeps h beside them.
+constexpr int64_t kMoeHLds = 64 * 1024;
+int moe_partial_bytes(int64_t tokens) { return (int)(tokens * 16 * 16 * 4); }
+int64_t moe_h_bytes(int64_t pairs, int64_t inter) { return 2 * pairs * (inter + 8) * 2; }
 
 // The kernels on `device` (current): loaded once per process and device, kept until the process ends.
 int kernels_on(const HostHip* hip, int device, const DeviceKernels** out) {
@@ -79,7 +86,7 @@ int kernels_on(const HostHip* hip, int device, const DeviceKernels** out) {
       // a block of the experts' second kernel may use more than 64 KiB of LDS, part of it dynamic
       if (e == hipSuccess && i >= kMoeDown)
         e = hip->FuncSetAttribute ? hip->FuncSetAttribute((const void*)k->fn[i], hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                          moe_partial_bytes(MOE_T, MOE_K))
+                                                          moe_partial_bytes(MOE_T) + (int)kMoeHLds)
                                   : hipErrorNotSupported;
     }
     if (e != hipSuccess) {
@@ -232,9 +239,11 @@ int kcg_matmul_fp8(const kcg_matmul_fp8_args* p, int device, uint64_t stream) {
   int fn, block;
   int64_t blocks;
   if (p->m <= 64) {
-    fn = kSkinny + t * 3 + (p->m <= 16 ? 0 : p->m <= 32 ? 1 : 2);
-    block = 512;
-    blocks = (p->n + 15) / 16;
+    // 32 rows of b a block where that still fills the chip: 37 x 8192 x 4096 takes 12.5 us so, 18.8 with 16 rows
+    const int rt = p->n >= 32 * 224 ? 2 : 1;
+    fn = kSkinny + t * 8 + (int)(p->m - 1) / 16 * 2 + rt - 1;
+    block = SKINNY_WAVES * 64;
+    blocks = (p->n + 16 * rt - 1) / (16 * rt);
   } else {
     static const int edge[3] = {256, 128, 64}, threads[3] = {512, 256, 256};
     static const int first[3] = {kTile, kTile + 2, kTile + 5};
@@ -257,8 +266,7 @@ int64_t kcg_moe_workspace_bytes(int64_t tokens, int64_t experts, int64_t topk, i
   if (topk < 1 || topk > MOE_K || topk > experts) return bad("moe_layer: topk must be in [1, 16] and at most experts");
   if (hidden < 16 || hidden % 16 || hidden > (1 << 20) || inter < 16 || inter % 16 || inter > (1 << 20))
     return bad("moe_layer: hidden and inter must be multiples of 16, at most 2^20");
-  const int64_t slots = tokens * topk < experts ? tokens * topk : experts;
-  const int64_t bytes = 2 * (tokens * topk * inter * 2) + slots * MOE_SLOT * 4 + tokens * topk * 4;
+  const int64_t bytes = 2 * (tokens * topk * inter * 2) + tokens * topk * 4;
   return (bytes + 15) / 16 * 16;
 }
 
@@ -290,13 +298,23 @@ int kcg_moe_layer(const kcg_moe_layer_args* p, int device, uint64_t stream) {
   char* ws = (char*)p->workspace;
   const int64_t plane = pairs * p->inter * 2;
   MoeArgs a = {(const void*)p->x, (const float*)p->logits, (const void*)p->w13, (const void*)p->w2, (const float*)p->w13_scale, (const float*)p->w2_scale,
-               (void*)p->out, (int32_t*)p->ids, (float*)p->probs, ws, ws + plane, (int32_t*)(ws + 2 * plane),
-               (float*)(ws + 2 * plane + slots * MOE_SLOT * 4), p->x_stride, p->logits_stride, p->out_stride, p->w13_stride_expert,
+               (void*)p->out, (int32_t*)p->ids, (float*)p->probs, ws, ws + plane, (float*)(ws + 2 * plane), p->x_stride, p->logits_stride, p->out_stride, p->w13_stride_expert,
                p->w13_stride_row, p->w2_stride_expert, p->w2_stride_row, (int)p->tokens, (int)p->experts, (int)p->topk, (int)p->hidden,
-               (int)p->inter, (int)slots, p->renormalize != 0};
+               (int)p->inter, (int)slots, p->renormalize != 0, UP_WAVES, 1};
+  // Waves that share 16 rows of the first product: as few as leave 4096 waves to the chip, two at least (at 64 tokens, 128
+  // experts of 1024 x 4096: 220 us with one, 196 with two, 215 with four, 260 with eight; at one token, 8 of 64 experts
+  // of 1024 x 2048: 23.2, 14.8, 10.4 and 9.9).
+  const int64_t row_groups = p->inter / 16;
+  a.split = 2;
+  while (a.split < UP_WAVES && row_groups * slots * a.split < 4096) a.split *= 2;
+  const int per_block = UP_WAVES / a.split;
+  // the second kernel keeps h in LDS where it fits (one token, 8 experts of 1024: 12.7 us without)
+  const int64_t h_bytes = moe_h_bytes(pairs, p->inter);
+  const int in_lds = h_bytes <= kMoeHLds;
   return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) {
-    if (int rc = launch(hip, k.fn[kMoeUp + v], (unsigned)(p->inter / 16), (unsigned)slots, UP_WAVES * 64, 0, stream, &a)) return rc;
-    return launch(hip, k.fn[kMoeDown + v], (unsigned)(p->hidden / 16), 1, DOWN_WAVES * 64, moe_partial_bytes(p->tokens, p->topk), stream, &a);
+    if (int rc = launch(hip, k.fn[kMoeUp + v], (unsigned)((row_groups + per_block - 1) / per_block), (unsigned)slots, UP_WAVES * 64, 0, stream, &a)) return rc;
+    return launch(hip, k.fn[kMoeDown + 2 * v + in_lds], (unsigned)(p->hidden / 16), 1, DOWN_WAVES * 64,
+                  moe_partial_bytes(p->tokens) + (in_lds ? (int)h_bytes : 0), stream, &a);
   });
 }
 

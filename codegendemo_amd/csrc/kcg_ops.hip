@@ -20,18 +20,20 @@ SWIGLU(__bf16, bf16)
 SWIGLU(_Float16, f16)
 SWIGLU(float, f32)
 
-#define SKINNY(TC, NAME, CT, NW)                                                                     \
-  extern "C" __global__ void __launch_bounds__(NW * 64) kcg_mm8_skinny_##NAME##_##CT(MatmulArgs a) { \
-    __shared__ f32x4 red[NW * CT * 64];                                                              \
-    skinny_kernel<TC, CT, NW>(a, (float*)red);                                                       \
+#define SKINNY(TC, NAME, CT, RT)                                                                              \
+  extern "C" __global__ void __launch_bounds__(SKINNY_WAVES * 64) kcg_mm8_skinny_##NAME##_##CT##x##RT(MatmulArgs a) { \
+    __shared__ f32x4 red[SKINNY_WAVES * CT * RT * 64];                                                         \
+    skinny_kernel<TC, CT, RT, SKINNY_WAVES>(a, red);                                                           \
   }
+#define SKINNIES(TC, NAME) \
+  SKINNY(TC, NAME, 1, 1) SKINNY(TC, NAME, 1, 2) SKINNY(TC, NAME, 2, 1) SKINNY(TC, NAME, 2, 2) SKINNY(TC, NAME, 3, 1) SKINNY(TC, NAME, 3, 2) SKINNY(TC, NAME, 4, 1) SKINNY(TC, NAME, 4, 2)
 #define TILE(TC, NAME, BM, BN, WM, WN, WPE)                                                                            \
   extern "C" __global__ void __launch_bounds__(WM * WN * 64, WPE) kcg_mm8_tile_##NAME##_##BM##x##BN(MatmulArgs a) {     \
     __shared__ __attribute__((aligned(1024))) uint8_t smem[TilePlan<TC, BM, BN, WM, WN>::LDS];                         \
     tile_kernel<TC, BM, BN, WM, WN>(a, smem);                                                                          \
   }
 #define MATMULS(TC, NAME) \
-  SKINNY(TC, NAME, 1, 8) SKINNY(TC, NAME, 2, 8) SKINNY(TC, NAME, 4, 8) TILE(TC, NAME, 128, 128, 2, 2, 2) TILE(TC, NAME, 64, 64, 2, 2, 2)
+  SKINNIES(TC, NAME) TILE(TC, NAME, 128, 128, 2, 2, 2) TILE(TC, NAME, 64, 64, 2, 2, 2)
 MATMULS(__bf16, bf16)
 MATMULS(_Float16, f16)
 MATMULS(float, f32)
@@ -39,10 +41,14 @@ TILE(__bf16, bf16, 256, 256, 4, 2, 2)
 TILE(_Float16, f16, 256, 256, 4, 2, 2)
 
 #define MOE(OPS, W, X, NAME)                                                                                        \
-  extern "C" __global__ void __launch_bounds__(UP_WAVES * 64) kcg_moe_up_##NAME(MoeArgs a) { up_kernel<OPS, W, X>(a); } \
-  extern "C" __global__ void __launch_bounds__(DOWN_WAVES * 64) kcg_moe_down_##NAME(MoeArgs a) {                    \
+  extern "C" __global__ void __launch_bounds__(UP_WAVES * 64, 4) kcg_moe_up_##NAME(MoeArgs a) { up_kernel<OPS, W, X>(a); } \
+  extern "C" __global__ void __launch_bounds__(DOWN_WAVES * 64) kcg_moe_down_##NAME##_0(MoeArgs a) {                \
     extern __shared__ __attribute__((aligned(16))) float partial[];                                                 \
-    down_kernel<W, X>(a, partial);                                                                                  \
+    down_kernel<W, X, false>(a, partial);                                                                           \
+  }                                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(DOWN_WAVES * 64) kcg_moe_down_##NAME##_1(MoeArgs a) {                \
+    extern __shared__ __attribute__((aligned(16))) float partial[];                                                 \
+    down_kernel<W, X, true>(a, partial);                                                                            \
   }
 MOE(Bf16Ops, uint8_t, __bf16, e4m3_bf16)
 MOE(F16Ops, uint8_t, _Float16, e4m3_f16)

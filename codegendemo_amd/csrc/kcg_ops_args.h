@@ -39,10 +39,12 @@ struct MatmulArgs {
   int grid_m, grid_n;        // tiles (tile kernel)
 };
 
+constexpr int SKINNY_WAVES = 8;
+
 constexpr int MOE_T = 64;        // most tokens of a call of the experts' layer
 constexpr int MOE_E = 512;       // most experts
 constexpr int MOE_K = 16;        // most experts of a token
-constexpr int MOE_SLOT = 2 + MOE_T;
+constexpr int MOE_ITEMS = 640;   // most runs of up to 8 tokens of one expert: one per expert, and T k / 8 more
 constexpr int UP_WAVES = 8;
 constexpr int DOWN_WAVES = 16;
 
@@ -58,12 +60,12 @@ struct MoeArgs {
   float* probs;                // [T, k] out: their weights
   void* h_hi;                  // workspace: [T k, I] twice
   void* h_lo;
-  int32_t* table;              // workspace: slots x MOE_SLOT: tokens, expert, the slot's pairs (t k + place)
   float* picked;               // workspace: [T, k] logits of the chosen (renormalised) or their probabilities
   int64_t x_stride, logits_stride, out_stride;
   int64_t w13_e, w13_r, w2_e, w2_r;     // elements from expert to expert, row to row
   int T, E, k, H, I, slots;
   int renormalize;
+  int split, rounds;           // first kernel: waves that share 16 rows, sets of rows a block takes one after another
 };
 
 }  // namespace kcg_ops

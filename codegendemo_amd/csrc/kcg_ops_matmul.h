@@ -9,18 +9,21 @@
 namespace kcg_ops {
 
 // ---------------------------------------------------------------------------------------------
-// Few rows (M <= 16 CT): bound by the bytes of B.  A block owns 16 rows of B; its NW waves split K (wave w takes groups
-// w, w + NW, ...), every byte of B goes from memory straight into the matrix operand, 2 KiB per wave and load pair, and
-// the partial sums meet in LDS, added in wave order (the same result on every run).
+// Few rows (M <= 16 CT): bound by the bytes of B and, from some 16 rows on, by what its blocks read of A between them.  A
+// block owns 16 RT rows of B; its NW waves split K, every byte of B goes from memory straight into the matrix operand (an
+// instruction reads 64 bytes of 16 rows, the next one the rest of those lines), and the partial sums meet in LDS, added
+// in wave order (the same result on every run).  RT = 2 halves the reads of A for each byte of B.
 // ---------------------------------------------------------------------------------------------
-template <class TC, int CT, int NW>
-__device__ void skinny_kernel(const MatmulArgs& p, float* red) {
+template <class TC, int CT, int RT, int NW>
+__device__ void skinny_kernel(const MatmulArgs& p, f32x4* red) {
   typedef typename DotOf<TC>::type Dot;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const uint8_t* b = p.b + (int64_t)min(n0 + r, p.N - 1) * p.ldb;      // (rows beyond N: computed from a row that exists, not stored)
-  const float* sb = p.sb + (int64_t)(n0 / GROUP) * p.sb_n;
+  const int n0 = blockIdx.x * 16 * RT;
+  const uint8_t* b[RT];
+#pragma unroll
+  for (int q = 0; q < RT; ++q) b[q] = p.b + (int64_t)min(n0 + q * 16 + r, p.N - 1) * p.ldb;   // (rows beyond N: computed from one that exists, not stored)
+  const float* sb = p.sb + (int64_t)(n0 / GROUP) * p.sb_n;       // (16 RT rows from a multiple of 16 RT lie in one block of 128)
   const uint8_t* a[CT];
   const float* sa[CT];
 #pragma unroll
@@ -29,66 +32,69 @@ __device__ void skinny_kernel(const MatmulArgs& p, float* red) {
     a[t] = p.a + m * p.lda;
     sa[t] = p.sa + m * p.sa_m;
   }
-  f32x4 acc[CT];
+  f32x4 acc[RT][CT];
 #pragma unroll
-  for (int t = 0; t < CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto step = [&](const i32x8& bq, const i32x8 (&aq)[CT], const float (&s)[CT], float sbv) {
-    const typename Dot::frag bf = Dot::make(bq);
+  for (int q = 0; q < RT; ++q)
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-      const f32x4 d = Dot::mma(bf, Dot::make(aq[t]));
-      const float f = s[t] * sbv;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(d[i], f, acc[t][i]);
-    }
-  };
-  const int full = p.K / GROUP;
-  int kb = wave;
-  // U groups at a time, all their loads in front of the first product
-  constexpr int U = CT == 1 ? 4 : 2;
-  for (; kb + (U - 1) * NW < full; kb += U * NW) {
-    i32x8 bq[U], aq[U][CT];
+    for (int t = 0; t < CT; ++t) acc[q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // U groups from kb on, all their loads in front of the first product
+  auto groups = [&](auto u_c, auto whole_c, int kb) {
+    constexpr int U = decltype(u_c)::value;
+    constexpr bool WHOLE = decltype(whole_c)::value;
+    i32x8 bq[U][RT], aq[U][CT];
     float s[U][CT], sbv[U];
+    auto load = [&](const uint8_t* row, int k) {
+      if constexpr (WHOLE) return join(*(const u32x4_a*)(row + k), *(const u32x4_a*)(row + k + 64));
+      else return join(load16_masked(row, k, p.K), load16_masked(row, k + 64, p.K));
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int q = 0; q < RT; ++q) bq[u][q] = load(b[q], (kb + u) * GROUP + g * 16);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = (kb + u * NW) * GROUP + g * 32;
-      bq[u] = join(__builtin_nontemporal_load((const u32x4_a*)(b + k)), __builtin_nontemporal_load((const u32x4_a*)(b + k + 16)));
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = (kb + u * NW) * GROUP + g * 32;
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        aq[u][t] = join(*(const u32x4_a*)(a[t] + k), *(const u32x4_a*)(a[t] + k + 16));
-        s[u][t] = sa[t][(kb + u * NW) * p.sa_k];
+        aq[u][t] = load(a[t], (kb + u) * GROUP + g * 16);
+        s[u][t] = sa[t][(kb + u) * p.sa_k];
       }
-      sbv[u] = sb[(kb + u * NW) * p.sb_k];
+      sbv[u] = sb[(kb + u) * p.sb_k];
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) step(bq[u], aq[u], s[u], sbv[u]);
-  }
-  for (; kb < p.KB; kb += NW) {                    // the rest, the partial last group among it
-    const int k = kb * GROUP + g * 32;
-    const i32x8 bq = join(load16_masked(b, k, p.K), load16_masked(b, k + 16, p.K));
-    i32x8 aq[CT];
-    float s[CT];
+    for (int u = 0; u < U; ++u) {
+      typename Dot::frag bf[RT];
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-      aq[t] = join(load16_masked(a[t], k, p.K), load16_masked(a[t], k + 16, p.K));
-      s[t] = sa[t][kb * p.sa_k];
+      for (int q = 0; q < RT; ++q) bf[q] = Dot::make(bq[u][q]);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        const typename Dot::frag af = Dot::make(aq[u][t]);
+        const float f = s[u][t] * sbv[u];
+#pragma unroll
+        for (int q = 0; q < RT; ++q) {
+          const f32x4 d = Dot::mma(bf[q], af);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[q][t][i] = fmaf(d[i], f, acc[q][t][i]);
+        }
+      }
     }
-    step(bq, aq, s, sb[kb * p.sb_k]);
-  }
-  // red[wave][t][lane] of 4 floats
-  f32x4* red4 = (f32x4*)red;
+  };
+  constexpr int U = CT == 1 ? 4 : 2;
+  int kb = p.KB * wave / NW;
+  const int to = p.KB * (wave + 1) / NW, whole = min(to, p.K / GROUP);
+  for (; kb + U <= whole; kb += U) groups(Int<U>(), Int<1>(), kb);
+  for (; kb < to; ++kb) groups(Int<1>(), Int<0>(), kb);            // the rest, the partial last group among it
+  constexpr int TILES = RT * CT;
 #pragma unroll
-  for (int t = 0; t < CT; ++t) red4[(wave * CT + t) * 64 + lane] = acc[t];
+  for (int q = 0; q < RT; ++q)
+#pragma unroll
+    for (int t = 0; t < CT; ++t) red[(wave * TILES + q * CT + t) * 64 + lane] = acc[q][t];
   __syncthreads();
-  for (int i = threadIdx.x; i < CT * 64; i += NW * 64) {
-    f32x4 v = red4[i];
+  for (int i = threadIdx.x; i < TILES * 64; i += NW * 64) {
+    f32x4 v = red[i];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) v += red4[w * CT * 64 + i];
-    const int m = (i >> 6) * 16 + (i & 15), n = n0 + ((i >> 4) & 3) * 4;
+    for (int w = 1; w < NW; ++w) v += red[w * TILES * 64 + i];
+    const int tile = i >> 6, q = tile / CT, t = tile - q * CT;
+    const int m = t * 16 + (i & 15), n = n0 + q * 16 + ((i >> 4) & 3) * 4;
     if (m < p.M && n < p.N) store4((TC*)p.c + (int64_t)m * p.ldc + n, v, p.N - n, p.c_wide);
   }
 }

@@ -15,52 +15,69 @@
 
 namespace kcg_ops {
 
-// order of floats as order of unsigned integers; -0 counts as 0
+// order of floats as order of unsigned integers; -0 counts as 0; 0 is below every key
 __device__ __forceinline__ unsigned order_key(float v) {
-  if (v == 0.f) return 0x80000000u;
   const unsigned u = __float_as_uint(v);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  unsigned k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  if (v == 0.f) k = 0x80000000u;
+  if ((u & 0x7fffffffu) > 0x7f800000u) k = 0xffffffffu;
+  return k;
 }
 
-// A lane's 32 consecutive values of a group of 128 (values 32 g .. 32 g + 31 for lane l, g = l / 16) as four operands of 8.
-// `n` of the 32 exist (0, 16 or 32: the extents are multiples of 16), the others are zero.
-template <class Ops>
-struct Frag {
-  typename Ops::vec v[4];
-};
-template <class Ops>
-__device__ __forceinline__ Frag<Ops> load_weights(const uint8_t* p, int n) {
-  u32x4 a = {0u, 0u, 0u, 0u}, b = a;
-  if (n > 0) a = __builtin_nontemporal_load((const u32x4_a*)p);
-  if (n > 16) b = __builtin_nontemporal_load((const u32x4_a*)(p + 16));
-  Frag<Ops> f;
-  f.v[0] = Ops::widen(a[0], a[1]);
-  f.v[1] = Ops::widen(a[2], a[3]);
-  f.v[2] = Ops::widen(b[0], b[1]);
-  f.v[3] = Ops::widen(b[2], b[3]);
-  return f;
+// sums over the 8 lanes of an aligned eighth of a wave
+template <class T>
+__device__ __forceinline__ T sum8(T v) {
+  auto dpp = [](T x, auto ctrl) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  v += dpp(v, Int<0xB1>());      // quad_perm: lane ^ 1
+  v += dpp(v, Int<0x4E>());      // quad_perm: lane ^ 2
+  v += dpp(v, Int<0x141>());     // row_half_mirror: the other four
+  return v;
 }
-template <class Ops, class T>
-__device__ __forceinline__ Frag<Ops> load_values(const T* p, int n) {
-  u32x4 t[4];
+
+// ---- 16-bit operands from weights and values ---------------------------------------------------------
+// A group of 128 k values is four operands of 8 per lane.  Operand i of lane l (g = l / 16) holds the 8 values from
+// place(g, i) on, the same for weights and values: two loads of 16 bytes cover a line of 8-bit weights.
+template <class W>
+__device__ __forceinline__ constexpr int place(int g, int i) {
+  return sizeof(W) == 1 ? (i >> 1) * 64 + g * 16 + (i & 1) * 8 : i * 32 + g * 8;
+}
+template <class W> struct Raw {                       // weights as they are stored
+  u32x4 v[sizeof(W) == 1 ? 2 : 4];
+};
+struct RawValues {
+  u32x4 v[4];
+};
+// The loads have no branches (behind one, the compiler could not count which loads are in flight, and would wait for all of
+// them): a place at or behind `n` (a multiple of 16) is read from the row's last values instead, and clear_tail() makes the
+// weights there zero.
+template <class W>
+__device__ __forceinline__ Raw<W> load_w(const W* row, int k, int g, int n) {
+  Raw<W> q;
+  constexpr int C = sizeof(W) == 1 ? 2 : 4;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) t[i] = n > 8 * i ? *(const u32x4_u*)(p + 8 * i) : u32x4{0u, 0u, 0u, 0u};
-  Frag<Ops> f;
+  for (int i = 0; i < C; ++i) q.v[i] = *(const u32x4_a*)(row + min(k + place<W>(g, i * (4 / C)), n - 16 / (int)sizeof(W)));
+  return q;
+}
+template <class W, class X>
+__device__ __forceinline__ RawValues load_x(const X* row, int k, int g, int n) {
+  RawValues q;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f.v[i] = __builtin_bit_cast(typename Ops::vec, t[i]);
-  return f;
+  for (int i = 0; i < 4; ++i) q.v[i] = *(const u32x4_u*)(row + min(k + place<W>(g, i), n - 8));
+  return q;
+}
+template <class W>
+__device__ __forceinline__ void clear_tail(Raw<W>& q, int k, int g, int n) {
+  constexpr int C = sizeof(W) == 1 ? 2 : 4;
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (k + place<W>(g, i * (4 / C)) >= n) q.v[i] = u32x4{0u, 0u, 0u, 0u};
 }
 template <class Ops, class W>
-__device__ __forceinline__ Frag<Ops> load_w(const W* p, int n) {
-  if constexpr (sizeof(W) == 1) return load_weights<Ops>((const uint8_t*)p, n);
-  else return load_values<Ops, W>(p, n);
-}
-template <class Ops>
-__device__ __forceinline__ f32x4 mma32(const Frag<Ops>& a, const Frag<Ops>& b, f32x4 c) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c = Ops::mma(a.v[i], b.v[i], c);
-  return c;
+__device__ __forceinline__ typename Ops::vec operand(const Raw<W>& q, int i) {
+  if constexpr (sizeof(W) == 1) return Ops::widen(q.v[i >> 1][2 * (i & 1)], q.v[i >> 1][2 * (i & 1) + 1]);
+  else return __builtin_bit_cast(typename Ops::vec, q.v[i]);
 }
 __device__ __forceinline__ void add_scaled(f32x4& acc, const f32x4& d, float s) {
 #pragma unroll
@@ -69,58 +86,98 @@ __device__ __forceinline__ void add_scaled(f32x4& acc, const f32x4& d, float s) 
 
 // ---- routing: which expert this block's slot serves, and for which tokens ----------------------------
 struct RouteLds {
-  unsigned key[MOE_E];
   int rank[MOE_T];             // the expert's place among the token's logits, -1: not chosen
   int token[MOE_T];            // the tokens that chose it, rising
-  int expert, count;
 };
 
-// Slots: with T k <= E one per (token, place), the first token that chose an expert serves all of its tokens and the other
+// The expert in place `place` of one token's logits (in every lane): the largest, taken out `place` times.
+__device__ __forceinline__ int expert_in_place(const float* l, int E, int place) {
+  const int lane = threadIdx.x & 63;
+  unsigned key[MOE_E / 64];
+#pragma unroll
+  for (int i = 0; i < MOE_E / 64; ++i) key[i] = i * 64 + lane < E ? order_key(l[i * 64 + lane]) : 0u;
+  int e = 0;
+  for (int n = 0;; ++n) {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < MOE_E / 64; ++i)
+      if (i * 64 < E) m = max(m, key[i]);
+    m = row_umax(m);
+    m = max(max((unsigned)__builtin_amdgcn_readlane(m, 0), (unsigned)__builtin_amdgcn_readlane(m, 16)),
+            max((unsigned)__builtin_amdgcn_readlane(m, 32), (unsigned)__builtin_amdgcn_readlane(m, 48)));
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < MOE_E / 64; ++i)
+      if (i * 64 < E && !found) {
+        const unsigned long long who = __ballot(key[i] == m);
+        if (who) {
+          found = true;
+          const int at = __ffsll(who) - 1;
+          e = i * 64 + at;
+          if (lane == at) key[i] = 0;
+        }
+      }
+    if (n == place) return e;
+  }
+}
+
+// Slots: with T k < E one per (token, place), the first token that chose an expert serves all of its tokens and the other
 // slots of that expert stay empty; else one per expert.  Returns the number of tokens (the same in every thread).
-__device__ __forceinline__ int route(const MoeArgs& a, RouteLds& s, int slot, bool designated) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int first = 0;
+__device__ __forceinline__ int route(const MoeArgs& a, RouteLds& s, int slot, bool designated, int& expert) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int first = 0, ex = slot;
   if (a.slots < a.E) {
     first = slot / a.k;
-    const int place = slot - first * a.k;
-    const float* l = a.logits + (int64_t)first * a.logits_stride;
-    unsigned mine = 0;
-    if (tid < a.E) s.key[tid] = mine = order_key(l[tid]);
-    __syncthreads();
-    if (tid < a.E) {
-      int n = 0;
-      for (int e = 0; e < a.E; ++e) {
-        const unsigned other = s.key[e];
-        n += (other > mine || (other == mine && e < tid)) ? 1 : 0;
+    ex = expert_in_place(a.logits + (int64_t)first * a.logits_stride, a.E, slot - first * a.k);
+  }
+  expert = ex;
+  if (a.T == 1 && a.slots < a.E && (a.renormalize || !designated)) {
+    // a token alone: the slot's place is all there is to know
+    if (lane == 0) {
+      s.rank[0] = slot;
+      s.token[0] = 0;
+      if (designated && wave == 0) {
+        a.ids[slot] = ex;
+        a.picked[slot] = a.logits[ex];
       }
-      if (n == place) s.expert = tid;
     }
     __syncthreads();
-  } else if (tid == 0) {
-    s.expert = slot;
+    return 1;
   }
-  if (a.slots >= a.E) __syncthreads();
-  const int ex = s.expert;
-  for (int t = wave; t < a.T; t += UP_WAVES) {
+  // 8 lanes a token, 8 tokens a wave
+  const int t = wave * 8 + (lane >> 3);
+  if (t < a.T) {
     const float* l = a.logits + (int64_t)t * a.logits_stride;
     const float lex = l[ex];
     const unsigned mine = order_key(lex);
+    const bool sums = designated && !a.renormalize;
     int n = 0;
     float sum = 0.f;
-    for (int e = lane; e < a.E; e += 64) {
-      const float le = l[e];
-      const unsigned other = order_key(le);
-      n += (other > mine || (other == mine && e < ex)) ? 1 : 0;
-      if (designated && !a.renormalize) sum += expf(le - lex);
-    }
-    // (n <= 512: nine bits a lane)
+#pragma unroll 4
+    for (int e = (lane & 7) * 4; e < a.E; e += 32) {
+      float v[4];
+      if (e + 4 <= a.E) {
+        typedef f32x4 __attribute__((may_alias, aligned(4))) V;
+        const f32x4 q = *(const V*)(l + e);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+        for (int i = 0; i < 4; ++i) v[i] = q[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = e + i < a.E ? l[e + i] : -__builtin_inff();
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned other = order_key(v[i]);
+        n += e + i < a.E && (other > mine || (other == mine && e + i < ex)) ? 1 : 0;
+        if (sums) sum += expf(v[i] - lex);             // (behind E: exp(-inf) = 0)
+      }
+    }
+    n = sum8(n);
     const bool chosen = n < a.k;
-    if (lane == 0) s.rank[t] = chosen ? n : -1;
+    if ((lane & 7) == 0) s.rank[t] = chosen ? n : -1;
     if (designated && chosen) {
-      if (!a.renormalize) sum = wave_sum(sum);
-      if (lane == 0) {
+      sum = sum8(sum);
+      if ((lane & 7) == 0) {
         const int pair = t * a.k + n;
         a.ids[pair] = ex;
         // softmax over all experts: 1 / sum exp(l' - l); an expert that is masked out (-inf) weighs nothing
@@ -129,243 +186,374 @@ __device__ __forceinline__ int route(const MoeArgs& a, RouteLds& s, int slot, bo
     }
   }
   __syncthreads();
-  if (wave == 0) {
-    const bool chosen = lane < a.T && s.rank[lane] >= 0;
-    const unsigned long long who = __ballot(chosen);
-    if (chosen) s.token[__popcll(who & ((1ull << lane) - 1))] = lane;
-    const bool again = a.slots < a.E && (who & ((1ull << first) - 1)) != 0;   // an earlier token's slot serves this expert
-    const int n = again ? 0 : __popcll(who);
-    if (lane == 0) s.count = n;
-    if (designated) {
-      int32_t* row = a.table + (int64_t)slot * MOE_SLOT;
-      if (lane == 0) {
-        row[0] = n;
-        row[1] = ex;
-      }
-      if (chosen) row[2 + __popcll(who & ((1ull << lane) - 1))] = lane * a.k + s.rank[lane];
-    }
-  }
-  __syncthreads();
-  return s.count;
+  // every wave for itself (and all write the same list)
+  const int rank = lane < a.T ? s.rank[lane] : -1;
+  const unsigned long long who = __ballot(rank >= 0);
+  if (rank >= 0) s.token[__popcll(who & ((1ull << lane) - 1))] = lane;
+  const bool again = a.slots < a.E && (who & ((1ull << first) - 1)) != 0;   // an earlier token's slot serves this expert
+  return again ? 0 : __popcll(who);
 }
 
 // ---- up ------------------------------------------------------------------------------------------
-// grid (I / 16, slots), UP_WAVES waves: 16 gate rows and the 16 up rows beside them; the waves split H by groups of 128 and
-// meet in LDS.
+// grid (x, slots), UP_WAVES waves.  A row group is 16 gate rows and the 16 up rows beside them.  `split` waves share a row
+// group, each with a part of H, and meet in LDS; UP_WAVES / split row groups run side by side, and a block takes `rounds` such
+// sets one after another.  split = 1 needs no barrier and lets every wave stream on its own: for calls with rows enough; a
+// single token's few rows take split = UP_WAVES.  The loads of a step (a group of 128 of one row group) are issued before the
+// products of the step in front of it, across row groups too (up to 16 tokens).
 template <class Ops, class W, class X, int CT>
-__device__ __forceinline__ void up_tiles(const MoeArgs& a, RouteLds& s, f32x4* red, int count) {
+__device__ __forceinline__ void up_tiles(const MoeArgs& a, RouteLds& s, f32x4* red, int ex, int count, int skip) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const int i0 = blockIdx.x * 16;
-  const int ex = __builtin_amdgcn_readfirstlane(s.expert);
-  const W* wg = (const W*)a.w13 + ex * a.w13_e + (int64_t)(i0 + r) * a.w13_r + g * 32;
-  const W* wu = wg + (int64_t)a.I * a.w13_r;
-  const int KB = (a.H + GROUP - 1) / GROUP;
-  const float* sg = nullptr;
-  const float* su = nullptr;
-  if constexpr (sizeof(W) == 1) {
-    const int rb = (2 * a.I + GROUP - 1) / GROUP;
-    sg = a.s13 + ((int64_t)ex * rb + i0 / GROUP) * KB;             // (16 rows from a multiple of 16 lie in one block)
-    su = a.s13 + ((int64_t)ex * rb + (a.I + i0) / GROUP) * KB;
-  }
+  const int split = a.split, side = UP_WAVES / split;
+  const int rg_end = a.I / 16, rounds = a.rounds;
+  const int rg0 = blockIdx.x * side * rounds + wave / split, part = wave % split;
+  const W* wg = (const W*)a.w13 + ex * a.w13_e + (int64_t)r * a.w13_r;
+  const int KB = (a.H + GROUP - 1) / GROUP, full = a.H / GROUP;
+  const float* sc = sizeof(W) == 1 ? a.s13 + (int64_t)ex * ((2 * a.I + GROUP - 1) / GROUP) * KB : nullptr;
   const X* x[CT];
 #pragma unroll
-  for (int c = 0; c < CT; ++c) x[c] = (const X*)a.x + (int64_t)s.token[min(c * 16 + r, count - 1)] * a.x_stride + g * 32;
-  f32x4 ag[CT], au[CT];
+  for (int c = 0; c < CT; ++c) x[c] = (const X*)a.x + (int64_t)s.token[min(skip + c * 16 + r, count - 1)] * a.x_stride;
+  struct Stage {
+    Raw<W> g, u;
+    RawValues x[CT];
+    float vg, vu;
+  };
+  auto load = [&](Stage& st, int rg, int kb) {
+    const W* rowg = wg + (int64_t)rg * 16 * a.w13_r;
+    const W* rowu = rowg + (int64_t)a.I * a.w13_r;
+    st.g = load_w<W>(rowg, kb * GROUP, g, a.H);
+    st.u = load_w<W>(rowu, kb * GROUP, g, a.H);
 #pragma unroll
-  for (int c = 0; c < CT; ++c) ag[c] = au[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto step = [&](int kb, int n) {
-    const Frag<Ops> fg = load_w<Ops>(wg + kb * GROUP, n), fu = load_w<Ops>(wu + kb * GROUP, n);
-    float vg = 1.f, vu = 1.f;
+    for (int c = 0; c < CT; ++c) st.x[c] = load_x<W>(x[c], kb * GROUP, g, a.H);
     if constexpr (sizeof(W) == 1) {
-      vg = sg[kb];
-      vu = su[kb];
+      // (16 rows from a multiple of 16 lie in one block of 128)
+      st.vg = sc[(int64_t)(rg * 16 / GROUP) * KB + kb];
+      st.vu = sc[(int64_t)((a.I + rg * 16) / GROUP) * KB + kb];
+    }
+  };
+  auto write = [&](int n, int row, float gate, float up) {
+    const int t = s.token[n];
+    const int64_t o = (int64_t)(t * a.k + s.rank[t]) * a.I + row;
+    const float h = gate / (1.f + expf(-gate)) * up;
+    const __bf16 hi = (__bf16)h;
+    const float hf = (float)hi;
+    ((__bf16*)a.h_hi)[o] = hi;
+    ((__bf16*)a.h_lo)[o] = __builtin_isfinite(hf) ? (__bf16)(h - hf) : (__bf16)0.f;
+  };
+  f32x4 ag[CT], au[CT];
+  auto start = [&]() {
+#pragma unroll
+    for (int c = 0; c < CT; ++c) ag[c] = au[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  auto multiply = [&](Stage& st, int kb) {
+    if (kb >= full) {
+      clear_tail<W>(st.g, kb * GROUP, g, a.H);
+      clear_tail<W>(st.u, kb * GROUP, g, a.H);
+    }
+    f32x4 dg[CT], du[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      dg[c] = sizeof(W) == 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : ag[c];
+      du[c] = sizeof(W) == 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : au[c];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const typename Ops::vec fg = operand<Ops, W>(st.g, i), fu = operand<Ops, W>(st.u, i);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const typename Ops::vec fx = __builtin_bit_cast(typename Ops::vec, st.x[c].v[i]);
+        dg[c] = Ops::mma(fg, fx, dg[c]);
+        du[c] = Ops::mma(fu, fx, du[c]);
+      }
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      const Frag<Ops> fx = load_values<Ops, X>(x[c] + kb * GROUP, n);
       if constexpr (sizeof(W) == 1) {
-        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        add_scaled(ag[c], mma32(fg, fx, z), vg);
-        add_scaled(au[c], mma32(fu, fx, z), vu);
+        add_scaled(ag[c], dg[c], st.vg);
+        add_scaled(au[c], du[c], st.vu);
       } else {
-        ag[c] = mma32(fg, fx, ag[c]);
-        au[c] = mma32(fu, fx, au[c]);
+        ag[c] = dg[c];
+        au[c] = du[c];
       }
     }
   };
-  const int full = a.H / GROUP;
-  int kb = wave;
-#pragma unroll 2
-  for (; kb < full; kb += UP_WAVES) step(kb, 32);
-  if (kb < KB) step(kb, min(32, a.H - kb * GROUP - g * 32));
+  // the sums of a row group become h
+  auto finish = [&](int round, int rg) {
+    if (split == 1) {
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    if (c) __syncthreads();
-    red[wave * 128 + lane] = ag[c];
-    red[wave * 128 + 64 + lane] = au[c];
-    __syncthreads();
-    if (tid < 256) {
-      // thread -> row tid % 16 of column tid / 16; element (row % 4) of the lane that holds it
-      const int row = tid & 15, col = tid >> 4, at = (row >> 2) * 16 + col;
-      float gate = 0.f, up = 0.f;
+      for (int c = 0; c < CT; ++c) {
+        const int n = skip + c * 16 + r;
+        if (n < count) {
 #pragma unroll
-      for (int w = 0; w < UP_WAVES; ++w) {
-        gate += red[w * 128 + at][row & 3];
-        up += red[w * 128 + 64 + at][row & 3];
+          for (int i = 0; i < 4; ++i) write(n, rg * 16 + g * 4 + i, ag[c][i], au[c][i]);
+        }
       }
-      const int n = c * 16 + col;
-      if (n < count) {
-        const int t = s.token[n];
-        const int64_t o = (int64_t)(t * a.k + s.rank[t]) * a.I + i0 + row;
-        const float h = gate / (1.f + expf(-gate)) * up;
-        const __bf16 hi = (__bf16)h;
-        const float hf = (float)hi;
-        ((__bf16*)a.h_hi)[o] = hi;
-        ((__bf16*)a.h_lo)[o] = __builtin_isfinite(hf) ? (__bf16)(h - hf) : (__bf16)0.f;
+    } else {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        __syncthreads();                              // (the sums of the tile before have been read)
+        red[wave * 128 + lane] = ag[c];
+        red[wave * 128 + 64 + lane] = au[c];
+        __syncthreads();
+        // thread -> row % 16 of column / 16 of a row group; element (row % 4) of the lane that holds it
+        for (int i = tid; i < side * 256; i += UP_WAVES * 64) {
+          const int q = i >> 8, row = i & 15, col = (i >> 4) & 15, at = (row >> 2) * 16 + col;
+          float gate = 0.f, up = 0.f;
+          for (int w = q * split; w < (q + 1) * split; ++w) {
+            gate += red[w * 128 + at][row & 3];
+            up += red[w * 128 + 64 + at][row & 3];
+          }
+          const int n = skip + c * 16 + col, to_rg = blockIdx.x * side * rounds + round * side + q;
+          if (n < count && to_rg < rg_end) write(n, to_rg * 16 + row, gate, up);
+        }
       }
+    }
+  };
+  const int from = KB * part / split, to = KB * (part + 1) / split;
+  // Every wave runs the same number of rounds, row groups behind the last one among them (there are barriers inside; such a
+  // row group is computed from the last one's weights and not stored).
+  int round = 0, kb = from;                            // of the next products
+  auto step = [&](Stage& st) {
+    if (kb == from) start();
+    multiply(st, kb);
+    if (++kb == to) {
+      const int rg = rg0 + round * side;
+      if (split > 1 || rg < rg_end) finish(round, rg);
+      ++round;
+      kb = from;
+    }
+  };
+  int load_round = 0, load_kb = from;
+  auto fetch = [&](Stage& st) {
+    load(st, min(rg0 + load_round * side, rg_end - 1), load_kb);
+    if (++load_kb == to) {
+      ++load_round;
+      load_kb = from;
+    }
+  };
+  int left = rounds * (to - from);
+  if (left == 0) {
+    for (; round < rounds; ++round) {
+      start();
+      if (split > 1) finish(round, rg0 + round * side);
+    }
+    return;
+  }
+  if constexpr (CT == 1) {
+    // (two named stages in turn: copying one into the other would wait for its loads)
+    Stage a0, a1;
+    fetch(a0);
+    for (; left > 2; left -= 2) {
+      fetch(a1);
+      step(a0);
+      fetch(a0);
+      step(a1);
+    }
+    if (left == 2) {
+      fetch(a1);
+      step(a0);
+      step(a1);
+    } else {
+      step(a0);
+    }
+  } else {
+    // (two stages of two column tiles would not fit the registers of 16 waves a compute unit)
+    for (; left > 0; --left) {
+      Stage now;
+      fetch(now);
+      step(now);
     }
   }
 }
 
+// (more than 32 tokens of one expert: its weights are read once more for each further 32)
 template <class Ops, class W, class X>
 __device__ void up_kernel(const MoeArgs& a) {
   __shared__ RouteLds s;
   __shared__ f32x4 red[UP_WAVES * 128];
-  const int count = route(a, s, blockIdx.y, blockIdx.x == 0);
-  if (count == 0) return;
-  if (count <= 16) up_tiles<Ops, W, X, 1>(a, s, red, count);
-  else if (count <= 32) up_tiles<Ops, W, X, 2>(a, s, red, count);
-  else up_tiles<Ops, W, X, 4>(a, s, red, count);
+  int ex;
+  const int count = route(a, s, blockIdx.y, blockIdx.x == 0, ex);
+  ex = __builtin_amdgcn_readfirstlane(ex);
+  for (int skip = 0; skip < count; skip += 32) {
+    if (count - skip <= 16) up_tiles<Ops, W, X, 1>(a, s, red, ex, count, skip);
+    else up_tiles<Ops, W, X, 2>(a, s, red, ex, count, skip);
+  }
 }
 
 // ---- down ----------------------------------------------------------------------------------------
-// grid H / 16: a block makes 16 columns of every token's row.  Work items are (expert, part of I); the waves take them in
-// turn, put their partial sums side by side in LDS, and the sum over parts and places runs in a fixed order.
+// grid H / 16: a block makes 16 columns of every token's row.  Work items are (expert, up to 8 of its tokens, part of I): the
+// 16 columns of a product hold the upper parts of 8 tokens' h and beside them the lower ones, whose sums are added at the
+// end, so that a group of 128 costs four loads of h and not eight (the loads, not the bytes, are what limits here: eight took
+// 167 us where four of them left out took 129, at 128 experts of 4096 x 1024).  The waves take the items in turn, put their partial sums side by side in LDS, and the sum over parts and places runs in a fixed order.
 struct DownLds {
-  int base[MOE_E + 1];         // pairs in front of an active slot
-  int slot[MOE_E];             // the active slots
-  int spot[MOE_T * MOE_K];     // where a pair's partial sums stand
+  unsigned long long tokens[MOE_E];   // which tokens chose the expert
+  int first[MOE_E];            // pairs of the experts in front of it
+  short item_expert[MOE_ITEMS], item_first[MOE_ITEMS], item_count[MOE_ITEMS];   // up to 8 pairs of one expert
+  int pair[MOE_T * MOE_K];     // pairs (t k + place) by expert, then token
+  int spot[MOE_T * MOE_K];     // where a pair stands in that order
   float prob[MOE_T * MOE_K];
-  int wave_sum[2][16];
-  int active;
+  int wave_sum[DOWN_WAVES];
+  int items;
 };
 
-template <class W, int CT>
-__device__ __forceinline__ void down_item(const MoeArgs& a, const int32_t* row, int count, int base, int part, int parts, float* partial) {
-  const int lane = threadIdx.x & 63;
-  const int r = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int ex = __builtin_amdgcn_readfirstlane(row[1]);
-  const W* w = (const W*)a.w2 + ex * a.w2_e + (int64_t)(n0 + r) * a.w2_r + g * 32;
-  const int KB = (a.I + GROUP - 1) / GROUP;
-  const float* sc = nullptr;
-  if constexpr (sizeof(W) == 1) sc = a.s2 + ((int64_t)ex * ((a.H + GROUP - 1) / GROUP) + n0 / GROUP) * KB;
-  const __bf16* hi[CT];
-  const __bf16* lo[CT];
-#pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const int64_t at = (int64_t)row[2 + min(c * 16 + r, count - 1)] * a.I + g * 32;
-    hi[c] = (const __bf16*)a.h_hi + at;
-    lo[c] = (const __bf16*)a.h_lo + at;
-  }
-  f32x4 acc[CT];
-#pragma unroll
-  for (int c = 0; c < CT; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto step = [&](int kb, int n) {
-    const Frag<Bf16Ops> fw = load_w<Bf16Ops>(w + kb * GROUP, n);
-    float v = 1.f;
-    if constexpr (sizeof(W) == 1) v = sc[kb];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      const Frag<Bf16Ops> fh = load_values<Bf16Ops, __bf16>(hi[c] + kb * GROUP, n), fl = load_values<Bf16Ops, __bf16>(lo[c] + kb * GROUP, n);
-      if constexpr (sizeof(W) == 1) {
-        const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-        add_scaled(acc[c], mma32(fw, fh, mma32(fw, fl, z)), v);
-      } else {
-        acc[c] = mma32(fw, fh, mma32(fw, fl, acc[c]));
-      }
-    }
-  };
-  const int from = KB * part / parts, to = KB * (part + 1) / parts, full = min(to, a.I / GROUP);
-  int kb = from;
-#pragma unroll 2
-  for (; kb < full; ++kb) step(kb, 32);
-  if (kb < to) step(kb, min(32, a.I - kb * GROUP - g * 32));
-#pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const int n = c * 16 + r;
-    if (n < count) *(f32x4*)(partial + (((base + n) * parts + part) * 16 + g * 4)) = acc[c];
-  }
-}
-
-template <class W, class X>
+// HL: h of the whole call fits LDS (a token or two): the block copies it there once and the waves' loads are the weights
+// alone, four steps of them in flight; else h comes from memory beside the weights, two steps in flight.
+template <class W, class X, bool HL>
 __device__ void down_kernel(const MoeArgs& a, float* partial) {
   __shared__ DownLds s;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // the active slots, and how many pairs lie in front of each (slots <= 512 threads)
-  int n = tid < a.slots ? a.table[(int64_t)tid * MOE_SLOT] : 0;
-  {
-    const unsigned long long who = __ballot(n > 0);
-    int before = n;                                  // inclusive sum over the wave's lanes
+  const int pairs = a.T * a.k;                       // (at most as many as threads; experts at most half of that)
+  const int my_expert = tid < pairs ? a.ids[tid] : 0;
+  const float my_value = tid < pairs ? a.picked[tid] : 0.f;
+  if (tid < a.E) s.tokens[tid] = 0;
+  if (tid < pairs) s.prob[tid] = my_value;
+  __syncthreads();
+  if (tid < pairs) atomicOr(&s.tokens[my_expert], 1ull << (tid / a.k));
+  __syncthreads();
+  // the chosen experts' items side by side, and how many pairs lie in front of each expert
+  const int n = tid < a.E ? __popcll(s.tokens[tid]) : 0;
+  const int mine = (n + 7) / 8;                    // items of this thread's expert
+  int upto = n << 16 | mine;                         // inclusive sums over the wave's lanes, of pairs (<= 1024) and items (<= 512)
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(before, d);
-      before += lane >= d ? o : 0;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(upto, d);
+    upto += lane >= d ? o : 0;
+  }
+  if (lane == 63) s.wave_sum[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) upto += s.wave_sum[w];
+  if (n > 0) {
+    const int first = (upto >> 16) - n, at = (upto & 0xffff) - mine;
+    s.first[tid] = first;
+    for (int i = 0; i < mine; ++i) {
+      s.item_expert[at + i] = (short)tid;
+      s.item_first[at + i] = (short)(first + i * 8);
+      s.item_count[at + i] = (short)min(8, n - i * 8);
     }
-    if (lane == 63) {
-      s.wave_sum[0][wave] = __popcll(who);
-      s.wave_sum[1][wave] = before;
+  }
+  if (tid == DOWN_WAVES * 64 - 1) s.items = upto & 0xffff;
+  __syncthreads();
+  if (tid < pairs) {
+    const int spot = s.first[my_expert] + __popcll(s.tokens[my_expert] & ((1ull << (tid / a.k)) - 1));
+    s.pair[spot] = tid;
+    s.spot[tid] = spot;
+  }
+  // the weights of the pairs (place 0 holds a token's largest logit)
+  float prob = my_value;
+  if (a.renormalize && tid < pairs) {
+    const float* l = s.prob + tid / a.k * a.k;
+    const float top = l[0];
+    float sum = 0.f;
+    for (int j = 0; j < a.k; ++j) sum += l[j] == -__builtin_inff() ? 0.f : expf(l[j] - top);
+    prob = my_value == -__builtin_inff() ? 0.f : expf(my_value - top) / sum;
+  }
+  if (blockIdx.x == 0 && tid < pairs) a.probs[tid] = prob;
+  __syncthreads();
+  if (tid < pairs) s.prob[tid] = prob;               // (read behind the barrier in front of the last sum)
+  const int items = s.items;
+  const int KB = (a.I + GROUP - 1) / GROUP, full = a.I / GROUP;
+  const int parts = max(1, min(DOWN_WAVES / items, KB));
+  const int r = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
+  // LDS: the partial sums, then (HL) h: upper parts, then lower ones, rows 8 values longer than they are (other banks)
+  const int h_row = a.I + 8;
+  __bf16* h_lds = (__bf16*)(partial + pairs * parts * 16);
+  struct Stage {
+    Raw<W> w;
+    RawValues h;                                     // (HL: read when it is used)
+    const __bf16* row;
+    float v;
+    int kb, item;                                    // item: -1 - item in its last step
+  };
+  // where the loads of the wave's next step come from
+  const W* w = nullptr;
+  const float* sc = nullptr;
+  const __bf16* h = nullptr;
+  int item = wave, kb = 0, to = 0;
+  auto open = [&]() {
+    if (item >= items * parts) return;
+    const int which = item / parts, part = item - which * parts;
+    const int ex = __builtin_amdgcn_readfirstlane(s.item_expert[which]), first = __builtin_amdgcn_readfirstlane(s.item_first[which]);
+    const int count = __builtin_amdgcn_readfirstlane(s.item_count[which]);
+    w = (const W*)a.w2 + ex * a.w2_e + (int64_t)(n0 + r) * a.w2_r;
+    if constexpr (sizeof(W) == 1) sc = a.s2 + ((int64_t)ex * ((a.H + GROUP - 1) / GROUP) + n0 / GROUP) * KB;
+    const int pair = s.pair[first + min(r & 7, count - 1)];
+    if constexpr (HL) h = h_lds + (pair + (r < 8 ? 0 : pairs)) * h_row;
+    else h = (const __bf16*)(r < 8 ? a.h_hi : a.h_lo) + (int64_t)pair * a.I;
+    kb = KB * part / parts;
+    to = KB * (part + 1) / parts;
+  };
+  auto load = [&](Stage& st) {
+    st.w = load_w<W>(w, kb * GROUP, g, a.I);
+    if constexpr (HL) st.row = h;
+    else st.h = load_x<W>(h, kb * GROUP, g, a.I);
+    if constexpr (sizeof(W) == 1) st.v = sc[kb];
+    st.kb = kb;
+    st.item = item;
+    if (++kb == to) {
+      st.item = -1 - item;
+      item += DOWN_WAVES;
+      open();
+    }
+  };
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](Stage& st) {
+    if (st.kb >= full) clear_tail<W>(st.w, st.kb * GROUP, g, a.I);
+    if constexpr (HL) st.h = load_x<W>(st.row, st.kb * GROUP, g, a.I);
+    f32x4 d = sizeof(W) == 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d = Bf16Ops::mma(operand<Bf16Ops, W>(st.w, i), __builtin_bit_cast(bf16x8, st.h.v[i]), d);
+    if constexpr (sizeof(W) == 1) add_scaled(acc, d, st.v);
+    else acc = d;
+    if (st.item < 0) {
+      const int done = -1 - st.item, which = done / parts, part = done - which * parts;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(acc[i]), 0x128, 0xf, 0xf, false));   // row_ror:8
+      if (r < s.item_count[which]) *(f32x4*)(partial + (((s.item_first[which] + r) * parts + part) * 16 + g * 4)) = acc;
+      acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  // The loads of a step are issued N - 1 steps before its products, across items too (named stages in turn: copying one into
+  // another would wait for its loads).
+  int left = 0;
+  for (int i = wave; i < items * parts; i += DOWN_WAVES) {
+    const int part = i % parts;
+    left += KB * (part + 1) / parts - KB * part / parts;
+  }
+  constexpr int N = HL ? 4 : 2;
+  Stage st[N];
+  open();
+  static_for<0, N - 1>([&](auto i_c) {
+    if (decltype(i_c)::value < left) load(st[decltype(i_c)::value]);
+  });
+  if constexpr (HL) {
+    // (16 bytes a thread; rows of I values, I a multiple of 16)
+    const int per_row = a.I / 8, chunks = 2 * pairs * per_row;
+    for (int i = tid; i < chunks; i += DOWN_WAVES * 64) {
+      const int row = i / per_row, c = i - row * per_row;
+      const __bf16* from = (row < pairs ? (const __bf16*)a.h_hi + (int64_t)row * a.I : (const __bf16*)a.h_lo + (int64_t)(row - pairs) * a.I) + c * 8;
+      *(u32x4_a*)(h_lds + row * h_row + c * 8) = *(const u32x4_a*)from;
     }
     __syncthreads();
-    int at = 0, pairs = 0;
-    for (int w = 0; w < wave; ++w) {
-      at += s.wave_sum[0][w];
-      pairs += s.wave_sum[1][w];
-    }
-    if (n > 0) {
-      at += __popcll(who & ((1ull << lane) - 1));
-      const int base = pairs + before - n;
-      s.slot[at] = tid;
-      s.base[at] = base;
-      const int32_t* row = a.table + (int64_t)tid * MOE_SLOT + 2;
-      for (int i = 0; i < n; ++i) s.spot[row[i]] = base + i;
-    }
-    if (tid == DOWN_WAVES * 64 - 1) s.active = at + (n > 0 ? 1 : 0);
   }
-  // the weights of the pairs
-  if (tid < a.T) {
-    const float* l = a.picked + tid * a.k;
-    if (a.renormalize) {
-      const float top = l[0];                        // place 0 holds the largest
-      float sum = 0.f;
-      for (int j = 0; j < a.k; ++j) sum += l[j] == -__builtin_inff() ? 0.f : expf(l[j] - top);
-      for (int j = 0; j < a.k; ++j) s.prob[tid * a.k + j] = l[j] == -__builtin_inff() ? 0.f : expf(l[j] - top) / sum;
-    } else {
-      for (int j = 0; j < a.k; ++j) s.prob[tid * a.k + j] = l[j];
-    }
-    if (blockIdx.x == 0)
-      for (int j = 0; j < a.k; ++j) a.probs[tid * a.k + j] = s.prob[tid * a.k + j];
+  for (; left >= 2 * N - 1; left -= N) {
+    static_for<0, N>([&](auto i_c) {
+      constexpr int i = decltype(i_c)::value;
+      load(st[(i + N - 1) % N]);
+      multiply(st[i]);
+    });
   }
-  __syncthreads();
-  const int active = s.active;
-  const int KB = (a.I + GROUP - 1) / GROUP;
-  const int parts = max(1, min(DOWN_WAVES / active, KB));
-  for (int item = wave; item < active * parts; item += DOWN_WAVES) {
-    const int at = item / parts, part = item - at * parts;
-    const int32_t* row = a.table + (int64_t)s.slot[at] * MOE_SLOT;
-    const int count = __builtin_amdgcn_readfirstlane(row[0]), base = s.base[at];
-    if (count <= 16) down_item<W, 1>(a, row, count, base, part, parts, partial);
-    else if (count <= 32) down_item<W, 2>(a, row, count, base, part, parts, partial);
-    else down_item<W, 4>(a, row, count, base, part, parts, partial);
-  }
+  static_for<0, 2 * N - 2>([&](auto i_c) {
+    constexpr int i = decltype(i_c)::value;
+    if (i + N - 1 < left) load(st[(i + N - 1) % N]);
+    if (i < left) multiply(st[i % N]);
+  });
   __syncthreads();
   for (int i = tid; i < a.T * 16; i += DOWN_WAVES * 64) {
     const int t = i >> 4, c = i & 15;
     float sum = 0.f;
     for (int j = 0; j < a.k; ++j) {
       const float p = s.prob[t * a.k + j];
-      const float* v = partial + (int64_t)s.spot[t * a.k + j] * parts * 16 + c;
+      const float* v = partial + s.spot[t * a.k + j] * parts * 16 + c;
       float y = 0.f;
       for (int q = 0; q < parts; ++q) y += v[q * 16];
       if (p != 0.f) sum = fmaf(p, y, sum);           // (a weight of 0 adds nothing, not even 0 * infinity)
