@@ -230,8 +230,9 @@ int kcg_matmul_fp8(const kcg_matmul_fp8_args* p, int device, uint64_t stream) {
       !any_stride_ok(p->b_scale_stride_group))
     return bad("matmul_fp8: a stride of the scales is negative");
   // a tile addresses its rows with 32-bit offsets from its first one
-  if ((p->m > 1 && p->a_stride > (1 << 22)) || (p->n > 1 && p->b_stride > (1 << 22)) || (p->m > 1 && p->a_scale_stride_row > (1 << 20)))
-    return bad("matmul_fp8: rows of a, b or a_scale are more than 2^22 (2^20) elements apart");
+  if ((p->m > 1 && p->a_stride > (1 << 22)) || (p->n > 1 && p->b_stride > (1 << 22)) || (p->m > 1 && p->a_scale_stride_row > (1 << 20)) ||
+      (p->n > 128 && p->b_scale_stride_row > (1 << 24)) || (p->k > 128 && p->b_scale_stride_group > (1 << 24)))
+    return bad("matmul_fp8: rows of a or b are more than 2^22 elements apart, of a_scale more than 2^20, or scales of b more than 2^24");
   MatmulArgs a = {(const uint8_t*)p->a, (const uint8_t*)p->b, (const float*)p->a_scale, (const float*)p->b_scale, (void*)p->c,
                   p->m > 1 ? p->a_stride : 0, p->n > 1 ? p->b_stride : 0, p->c_stride, p->m > 1 ? p->a_scale_stride_row : 0, p->a_scale_stride_group,
                   p->b_scale_stride_row, p->b_scale_stride_group, (int)p->m, (int)p->n, (int)p->k, (int)groups(p->k), 0, 0, 0};

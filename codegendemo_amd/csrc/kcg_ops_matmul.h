@@ -101,36 +101,53 @@ __device__ void skinny_kernel(const MatmulArgs& p, f32x4* red) {
 
 // ---------------------------------------------------------------------------------------------
 // Tiles of BM x BN, WM x WN waves, K in steps of one group (128 bytes of a row).
-// LDS: two stages of BM + BN rows of 128 bytes, filled by global_load_lds (16 bytes a lane, no registers).  The chunk at
+// LDS: S stages of BM + BN rows of 128 bytes, filled by global_load_lds (16 bytes a lane, no registers).  The chunk at
 // place c of row r is chunk c ^ (r & 7) of that row: 8 lanes that read one chunk column of 8 rows touch all banks.
 // A wave keeps its activation fragments (MB x 16 columns) for a K step and streams the weight fragments (NB x 16 rows)
-// past them, one ahead.  The step of stage s ends (barrier, fetch of the stage after the next into s) in front of the last
-// weight row, whose fragments are in registers by then: the fetch has a whole step to land, the fragment reads of the
-// next step run under the last row's matrix instructions, and the fma of a row run under those of the row behind it.
+// past them, two ahead.  A step ends (barrier, fetch into the stage it has read) in front of the last weight row, whose
+// fragments are in registers by then: with S = 2 a fetch has most of a step to land, with more stages S - 1 steps; the
+// fragment reads of the next step run under the last row's matrix instructions, and the fma of a product under the next
+// two products.
+// Scales come the same way in chunks of 8 steps, a chunk ahead: read per lane and step where they are needed, from rows
+// of their own, they made 4096^3 take 88 us, with rows side by side 70.
 // ---------------------------------------------------------------------------------------------
-template <class TC, int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int S>
 struct TilePlan {
   static constexpr int NT = WM * WN * 64;
   static constexpr int MB = BM / WM / 16, NB = BN / WN / 16;
   static constexpr int ROWS = BM + BN, STAGE = ROWS * GROUP;
   static constexpr int FETCH = ROWS * 8 / NT;      // 16-byte chunks a thread fetches for a stage
   static constexpr int RPF = NT / 8;               // rows one fetch of all threads covers
-  static constexpr int LDS = 2 * STAGE;
-  static_assert(BM % RPF == 0 && BN % RPF == 0 && NB >= 2, "tile plan");
+  // Pieces of a fetch: LAST behind the barrier, the others over the first rows of the next step where the tile is large (all
+  // at once, its waves stand in front of the one address unit, 16 cycles an instruction, and the matrix cores behind them:
+  // 8192^3 488 us, so 478); small tiles wait for memory, not for the unit (2048^3 19.7 us, all at once 17.3).
+  static constexpr int LAST = NB > 4 ? 2 : FETCH;
+  static constexpr int PER_ROW = (FETCH - LAST + NB / 2 - 1) / (NB / 2);
+  static constexpr int SB = BN >= GROUP ? BN / GROUP : 1;              // blocks of 128 rows of B a tile has scales from
+  static constexpr int STEPS = 8;                                      // of a chunk of scales
+  static constexpr int SCALES = STEPS * BM + 64;                       // floats of one: [step][row], then [block][step]
+  static constexpr int LDS = S * STAGE + 2 * SCALES * 4;
+  static_assert(BM % RPF == 0 && BN % RPF == 0 && NB >= 2 && NB % 2 == 0 && (S & (S - 1)) == 0 && SB * STEPS <= 64, "tile plan");
+  static_assert(BN / WN <= GROUP && GROUP % (BN / WN) == 0, "a wave's rows of B lie in one block of 128");
+  static_assert(S == 2 || LAST == FETCH, "the waits count whole fetches");
+  static_assert(BM % 64 == 0 && STEPS * BM / 64 % (NT / 64) == 0, "scales: whole waves");
 };
 
-// 16 bytes a lane from base + off into 1 KiB of LDS from lds on.  In assembly, because the compiler would wait for every
+// 16 (4) bytes a lane from base + off into consecutive LDS from lds on.  In assembly, because the compiler would wait for every
 // such fetch in front of each later LDS read; the waits that are needed are written out in the kernel.  (No output
 // registers; vmcnt counts it, which makes the compiler's own waits stricter, never weaker.)
-__device__ __forceinline__ void fetch_lds(const uint8_t* base, unsigned off, unsigned lds) {
+__device__ __forceinline__ void fetch_lds16(const void* base, unsigned off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
+__device__ __forceinline__ void fetch_lds4(const void* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
 
-template <class TC, int BM, int BN, int WM, int WN>
+template <class TC, int BM, int BN, int WM, int WN, int S>
 __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
-  typedef TilePlan<TC, BM, BN, WM, WN> P;
+  typedef TilePlan<BM, BN, WM, WN, S> P;
   typedef typename DotOf<TC>::type Dot;
-  constexpr int MB = P::MB, NB = P::NB;
+  constexpr int MB = P::MB, NB = P::NB, NW = WM * WN;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM;
   const int r = lane & 15, g = lane >> 4;
@@ -148,9 +165,10 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
   const int gm = min(GM, p.grid_m - grp * GM);
   const int tm = grp * GM + in % gm, tn = in / gm;
   const int m0 = tm * BM, n0 = tn * BN;
+  const int KB = p.KB;
 
-  // fetch: thread -> row tid / 8 (+ RPF per further fetch), place tid % 8
-  const int frow = tid >> 3, fchunk = (tid & 7) ^ (frow & 7);     // (RPF is a multiple of 8: the swizzle is the same in every fetch)
+  // fetch: thread -> row tid / 8 (+ RPF per further piece), place tid % 8
+  const int frow = tid >> 3, fchunk = (tid & 7) ^ (frow & 7);     // (RPF is a multiple of 8: the swizzle is the same in every piece)
   const uint8_t* abase = p.a + (int64_t)m0 * p.lda;
   const uint8_t* bbase = p.b + (int64_t)n0 * p.ldb;
   constexpr int FA = BM / P::RPF, FB = BN / P::RPF;
@@ -161,24 +179,23 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
   for (int f = 0; f < FB; ++f) off[FA + f] = (unsigned)(min(frow + f * P::RPF, p.N - 1 - n0) * (unsigned)p.ldb) + fchunk * 16;
   const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
   const unsigned lds_wave = lds0 + wave * 1024;
-  const int KB = p.KB;
   // a chunk of the partial last group that lies behind K: the row's first chunk of that group instead (cleared in LDS later)
   const bool ragged = (p.K & (GROUP - 1)) != 0;
   const bool behind = ragged && fchunk * 16 >= (p.K & (GROUP - 1));
-  auto fetch = [&](int kb) {
+  auto fetch = [&](auto from_c, auto to_c, int kb) {       // pieces [from, to) of FETCH
     const unsigned back = behind && kb == KB - 1 ? fchunk * 16 : 0;
-    const unsigned to = lds_wave + (kb & 1) * P::STAGE;
+    const unsigned to = lds_wave + (kb & (S - 1)) * P::STAGE;
     const uint8_t* ak = abase + (int64_t)kb * GROUP;
     const uint8_t* bk = bbase + (int64_t)kb * GROUP;
-#pragma unroll
-    for (int f = 0; f < FA; ++f) fetch_lds(ak, off[f] - back, to + f * P::RPF * GROUP);
-#pragma unroll
-    for (int f = 0; f < FB; ++f) fetch_lds(bk, off[FA + f] - back, to + (BM + f * P::RPF) * GROUP);
+    static_for<decltype(from_c)::value, decltype(to_c)::value>([&](auto f_c) {
+      constexpr int f = decltype(f_c)::value;
+      fetch_lds16(f < FA ? ak : bk, off[f] - back, to + f * P::RPF * GROUP);
+    });
   };
   // zeros behind K in the stage of the partial last group
   auto clear_tail = [&](int kb) {
     const int kt = p.K & (GROUP - 1);
-    uint8_t* st = smem + (kb & 1) * P::STAGE;
+    uint8_t* st = smem + (kb & (S - 1)) * P::STAGE;
     for (int i = tid; i < P::ROWS * 8; i += P::NT) {
       const int row = i >> 3, c = i & 7;
       u32x4_a* at = (u32x4_a*)(st + row * GROUP + ((c ^ (row & 7)) << 4));
@@ -198,32 +215,35 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
   const unsigned sw0 = ((g ^ (r & 7)) << 4), sw1 = (((g + 4) ^ (r & 7)) << 4);
   const uint8_t* arow = smem + (wm * MB * 16 + r) * GROUP;
   const uint8_t* brow = smem + (BM + wn * NB * 16 + r) * GROUP;
-  auto frag = [&](const uint8_t* base, int i, int stage) {
-    const uint8_t* q = base + stage * P::STAGE + i * 16 * GROUP;
+  auto frag = [&](const uint8_t* base, int i, int kb) {
+    const uint8_t* q = base + (kb & (S - 1)) * P::STAGE + i * 16 * GROUP;
     return join(*(const u32x4_a*)(q + sw0), *(const u32x4_a*)(q + sw1));
   };
-  // scales: one of the activations per lane and column tile, one of the weights per 128 of the wave's rows of B
-  constexpr int SPAN = NB * 16;
-  constexpr int SB = SPAN >= GROUP ? SPAN / GROUP : 1;
-  const int nb0 = (n0 + wn * SPAN) / GROUP, nb_last = (p.N - 1) / GROUP;
-  unsigned sa_off[MB];
+  // scales of chunk c (steps 8 c .. 8 c + 7): an instruction fetches 64 rows of one step, the last one those of the weights
+  constexpr int STEPS = P::STEPS, PARTS = BM / 64;
+  const float* const scales = (const float*)(smem + S * P::STAGE);
+  auto fetch_scales = [&](int c) {
+    const unsigned to = lds0 + S * P::STAGE + (c & 1) * P::SCALES * 4;
 #pragma unroll
-  for (int j = 0; j < MB; ++j) sa_off[j] = (unsigned)min((wm * MB + j) * 16 + r, p.M - 1 - m0) * (unsigned)p.sa_m;
-  const float* sa_tile = p.sa + (int64_t)m0 * p.sa_m;
-  float sa_raw[MB], sb_raw[SB];
-  auto load_scales = [&](int kb) {
-#pragma unroll
-    for (int q = 0; q < SB; ++q) sb_raw[q] = p.sb[(int64_t)min(nb0 + q, nb_last) * p.sb_n + (int64_t)kb * p.sb_k];
-    const float* base = sa_tile + (int64_t)kb * p.sa_k;
-#pragma unroll
-    for (int j = 0; j < MB; ++j) sa_raw[j] = base[sa_off[j]];
+    for (int i = 0; i < STEPS * PARTS / NW; ++i) {
+      const int at = wave + i * NW, step = at / PARTS, part = at % PARTS;
+      const float* base = p.sa + (int64_t)m0 * p.sa_m + (int64_t)min(c * STEPS + step, KB - 1) * p.sa_k;
+      fetch_lds4(base, (unsigned)min(part * 64 + lane, p.M - 1 - m0) * (unsigned)p.sa_m * 4u, to + at * 256);
+    }
+    if (wave == 0) {
+      const float* base = p.sb + (int64_t)(n0 / GROUP) * p.sb_n + (int64_t)c * STEPS * p.sb_k;
+      const int block = min(min(lane / STEPS, P::SB - 1), (p.N - 1) / GROUP - n0 / GROUP), step = min(lane % STEPS, KB - 1 - c * STEPS);
+      fetch_lds4(base, (unsigned)block * (unsigned)p.sb_n * 4u + (unsigned)step * (unsigned)p.sb_k * 4u, to + STEPS * BM * 4);
+    }
   };
-  float s[SB][MB];
-  auto join_scales = [&]() {
+  const float* my_sa = scales + wm * MB * 16 + r;
+  const float* my_sb = scales + STEPS * BM + (n0 % GROUP + wn * NB * 16) / GROUP * STEPS;
+  float s[MB], s_next[MB], sb_next;
+  auto read_scales = [&](float (&v)[MB], int kb) {
+    const int chunk = ((kb / STEPS) & 1) * P::SCALES, step = kb % STEPS;
 #pragma unroll
-    for (int q = 0; q < SB; ++q)
-#pragma unroll
-      for (int j = 0; j < MB; ++j) s[q][j] = sa_raw[j] * sb_raw[q];
+    for (int j = 0; j < MB; ++j) v[j] = my_sa[chunk + step * BM + j * 16];
+    sb_next = my_sb[chunk + step];
   };
 
   f32x4 acc[NB][MB];
@@ -233,65 +253,82 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
     for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   if (KB > 0) {
-    load_scales(0);
-    fetch(0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    join_scales();
+    fetch_scales(0);
+    static_for<0, S - 1>([&](auto k_c) {
+      constexpr int k = decltype(k_c)::value;
+      if (k < KB) fetch(Int<0>(), Int<P::FETCH>(), k);
+    });
+    // (in order: the first stage and the scales in front of it have landed when no more than the other stages are left)
+    if (KB >= S - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * P::FETCH) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read_scales(s, 0);
+#pragma unroll
+    for (int j = 0; j < MB; ++j) s[j] *= sb_next;
     if (ragged && KB == 1) {
       clear_tail(0);
       __syncthreads();
     }
-    if (KB > 1) fetch(1);
-    i32x8 am[MB], bn[2];
+    if (S - 1 < KB) fetch(Int<0>(), Int<P::LAST>(), S - 1);
+    i32x8 am[MB], bn[4];                         // weight row i in place i % 4, two rows ahead of its products
 #pragma unroll
     for (int j = 0; j < MB; ++j) am[j] = frag(arow, j, 0);
     bn[0] = frag(brow, 0, 0);
+    bn[1] = frag(brow, 1, 0);
     // Products q = i MB + j run through d[q % 3]; the fma of a product follows the second product behind it, when its result is
     // there without a wait.
     f32x4 d[3];
     auto add = [&](auto q_c) {
       constexpr int q = decltype(q_c)::value, i = q / MB, j = q % MB;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[q % 3][e], s[i * 16 / GROUP][j], acc[i][j][e]);
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[q % 3][e], s[j], acc[i][j][e]);
       // (here, not behind the branches at the end of the step, where the compiler would gather them and keep every d until then)
       asm volatile("" : "+v"(acc[i][j]));
     };
 
     for (int kb = 0; kb < KB; ++kb) {
-      const int stage = kb & 1;
       const int nx = min(kb + 1, KB - 1);
       typename Dot::frag af[MB];
 #pragma unroll
       for (int j = 0; j < MB; ++j) af[j] = Dot::make(am[j]);
-      load_scales(nx);                            // (used a step later: the loads have the whole step)
+      // (behind the stages fetched so far, in front of the ones to come: the waits below cover them)
+      if (kb % STEPS == 1 && kb - 1 + STEPS < KB) fetch_scales(kb / STEPS + 1);
       static_for<0, NB>([&](auto i_c) {
         constexpr int i = decltype(i_c)::value;
         if constexpr (i == NB - 1) {
-          // every fragment of this stage is in registers or on its way; the next stage has had a step to land
-          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          // every fragment of this stage is in registers or on its way; the next stage has landed when no more than the S - 2
+          // behind it are left
+          if (S > 2 && kb + S - 1 < KB) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * P::FETCH) : "memory");
+          else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
+          read_scales(s_next, nx);
           if (ragged && kb + 1 == KB - 1) {
             clear_tail(kb + 1);
             __syncthreads();
           }
-          if (kb + 2 < KB) fetch(kb + 2);
+          if (kb + S < KB) fetch(Int<0>(), Int<P::LAST>(), kb + S);
+        } else if constexpr (P::LAST + i * P::PER_ROW < P::FETCH) {
+          constexpr int to = P::LAST + (i + 1) * P::PER_ROW;
+          if (kb + S - 1 < KB) fetch(Int<P::LAST + i * P::PER_ROW>(), Int<(to < P::FETCH ? to : P::FETCH)>(), kb + S - 1);
         }
-        if constexpr (i + 1 < NB) bn[(i + 1) & 1] = frag(brow, i + 1, stage);
-        const typename Dot::frag bf = Dot::make(bn[i & 1]);
+        if constexpr (i + 2 < NB) bn[(i + 2) % 4] = frag(brow, i + 2, kb);
+        const typename Dot::frag bf = Dot::make(bn[i % 4]);
         static_for<0, MB>([&](auto j_c) {
           constexpr int j = decltype(j_c)::value, q = i * MB + j;
           d[q % 3] = Dot::mma(bf, af[j]);
-          if constexpr (i == NB - 1) am[j] = frag(arow, j, nx & 1);      // (after the last step: the same stage again, unused)
+          if constexpr (i == NB - 1) am[j] = frag(arow, j, nx);          // (after the last step: the same stage again, unused)
+          if constexpr (i == NB - 1 && j == 0) bn[0] = frag(brow, 0, nx);
+          if constexpr (i == NB - 1 && j == (NB > 2 ? 1 : MB - 1)) bn[1] = frag(brow, 1, nx);   // (NB = 2: row 1 is this row)
           if constexpr (q >= 2) add(Int<q - 2>());
+          __builtin_amdgcn_sched_barrier(0);
         });
-        __builtin_amdgcn_sched_barrier(0);
       });
-      bn[0] = frag(brow, 0, nx & 1);
       add(Int<NB * MB - 2>());
       add(Int<NB * MB - 1>());
-      join_scales();
+#pragma unroll
+      for (int j = 0; j < MB; ++j) s[j] = s_next[j] * sb_next;
     }
   }
 #pragma unroll
@@ -301,7 +338,7 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
       TC* c = (TC*)p.c + (int64_t)m * p.ldc;
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const int n = n0 + wn * SPAN + i * 16 + g * 4;
+        const int n = n0 + wn * NB * 16 + i * 16 + g * 4;
         if (n < p.N) store4(c + n, acc[i][j], p.N - n, p.c_wide);
       }
     }
