@@ -7,7 +7,7 @@ import struct
 
 from . import _native
 
-EXPORTS = ("kcg_ops_load", "kcg_rmsnorm_quant", "kcg_swiglu_quant", "kcg_matmul_fp8", "kcg_moe_layer", "kcg_moe_workspace_bytes")
+EXPORTS = ("kcg_ops_load", "kcg_rmsnorm_quant", "kcg_swiglu_quant", "kcg_matmul_fp8", "kcg_matmul_fp8_kernel", "kcg_moe_layer", "kcg_moe_workspace_bytes")
 DT_E4M3 = 1
 RMSNORM_QUANT = struct.Struct("=18qd")      # kcg_rmsnorm_quant_args
 SWIGLU_QUANT = struct.Struct("=10q")        # kcg_swiglu_quant_args
@@ -29,6 +29,7 @@ def lib():
             getattr(L, name).argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_uint64]
         L.kcg_moe_workspace_bytes.argtypes = [ctypes.c_int64] * 5
         L.kcg_moe_workspace_bytes.restype = ctypes.c_int64
+        L.kcg_matmul_fp8_kernel.argtypes = [ctypes.c_int64] * 4 + [ctypes.c_char_p, ctypes.c_int]
         L.kcg_ops_load.argtypes = [ctypes.c_int]
         _ops = L
     return _ops
@@ -41,3 +42,10 @@ def load(device=0):
 
 def moe_workspace_bytes(tokens, experts, topk, hidden, inter):
     return _native.check(lib().kcg_moe_workspace_bytes(tokens, experts, topk, hidden, inter))
+
+
+def matmul_fp8_kernel(m, n, k, c_dtype):
+    """Name of the kernel that a product of these sizes runs (c_dtype: a code of EnumKernelDType)."""
+    buf = ctypes.create_string_buffer(256)
+    _native.check(lib().kcg_matmul_fp8_kernel(m, n, k, int(c_dtype), buf, len(buf)))
+    return buf.value.decode()

@@ -1,5 +1,7 @@
 // kcg_ops.cc — host side of the operators declared in include/kcg_ops.h: argument checks, the choice of a kernel, launches.
 #include <climits>
+#include <cmath>
+#include <cstdio>
 #include <cstring>
 #include <map>
 #include <memory>
@@ -24,22 +26,88 @@ using kcg::HostHip;
 using namespace kcg_ops;
 
 // ---- kernels ---------------------------------------------------------------------------------
-enum { kNorm = 0, kSwiglu = kNorm + 21, kSkinny = kSwiglu + 3, kTile = kSkinny + 24, kMoeUp = kTile + 8, kMoeDown = kMoeUp + 3, kNumKernels = kMoeDown + 6 };
+// The tiles of the 8-bit product (kcg_ops_matmul.h).  A call takes the one that this estimate of its time, in microseconds,
+// is smallest for: every round of blocks costs start + steps * step, where a round is one block on each of the 256 compute
+// units, or two where two fit one (step2: their step); steps = groups of 128 of K / ks.  Measured for 16-bit results at
+// N, K in {1024 .. 16384}; the estimates lie within 10 % of what was measured, some 20 % at the largest sizes.
+struct Tile {
+  const char* name;
+  int bm, bn, ks, threads;
+  float start, step, step2;
+};
+const Tile kTileTable[] = {
+    {"32x32_2x1x4", 32, 32, 4, 512, 1.6f, .39f, 0.f},       // 37 x 1024 x 4096: 6.9 us (64 x 64: 12.4)
+    {"64x32_4x1x2", 64, 32, 2, 512, 1.2f, .36f, 0.f},       // 37 x 8192 x 4096: 9.5 (32 x 32: 12.8, 64 x 64 by two: 10.8)
+    {"64x64_2x2x1", 64, 64, 1, 256, .4f, .305f, .52f},      // 512 x 4096 x 1024: 7.3 (by two: 10.8)
+    {"64x64_2x2x2", 64, 64, 2, 512, 1.9f, .43f, 0.f},       // 256 x 4096 x 4096: 11.3 (by one: 12.8)
+    {"128x128_4x2x1", 128, 128, 1, 512, 2.f, .575f, 0.f},   // 1024 x 4096 x 4096: 24.8 (4 waves: 28.1)
+    {"128x128_2x2x1", 128, 128, 1, 256, 1.6f, .655f, 1.1f}, // 2048 x 4096 x 4096: 39.2 (8 waves: 46.2)
+    {"256x256_4x2x1", 256, 256, 1, 512, 7.f, 1.55f, 0.f},   // 4096^3: 63.0 (128 x 128: 75.1); 16-bit results
+};
+constexpr int kTiles = sizeof(kTileTable) / sizeof(kTileTable[0]);
+constexpr double kLaunch = 2.3;
+
+double tile_estimate(const Tile& v, int64_t m, int64_t n, int64_t groups) {
+  const double tiles = (double)((m + v.bm - 1) / v.bm) * (double)((n + v.bn - 1) / v.bn), steps = (double)((groups + v.ks - 1) / v.ks);
+  if (v.step2 == 0.f) return kLaunch + std::ceil(tiles / 256) * (v.start + steps * v.step);
+  const double full = std::floor(tiles / 512), rest = tiles - 512 * full;
+  return kLaunch + full * (v.start + steps * v.step2) + (rest > 0 ? v.start + steps * (rest <= 256 ? v.step : v.step2) : 0);
+}
+// 17 to 32 rows without a tile (rt: 16-row tiles of b a block): N / 16 / rt blocks
+double skinny_estimate(int rt, int64_t n, int64_t groups) {
+  const double rounds = (double)((n + 16 * rt - 1) / (16 * rt)) / 256;
+  return 2.2 + groups * (rt == 1 ? .172 : .24) * (rounds > 1 ? rounds : 1);
+}
+
+enum { kNorm = 0, kSwiglu = kNorm + 21, kSkinny = kSwiglu + 3, kTile = kSkinny + 12, kMoeUp = kTile + 3 * kTiles, kMoeDown = kMoeUp + 3, kNumKernels = kMoeDown + 6 };
 
 std::string kernel_symbol(int i) {
   static const char* const types[3] = {"bf16", "f16", "f32"};
   static const char* const norm[7] = {"64_1", "128_1", "256_1", "512_1", "1024_1", "1024_2", "1024_0"};
-  static const char* const tile[8] = {"bf16_256x256", "f16_256x256", "bf16_128x128", "f16_128x128", "f32_128x128", "bf16_64x64", "f16_64x64", "f32_64x64"};
   static const char* const moe[3] = {"e4m3_bf16", "e4m3_f16", "bf16_bf16"};
   if (i < kSwiglu) return std::string("kcg_norm_") + types[i / 7] + "_" + norm[i % 7];
   if (i < kSkinny) return std::string("kcg_swiglu_") + types[i - kSwiglu];
   if (i < kTile) {
-    const int v = (i - kSkinny) % 8;
-    return std::string("kcg_mm8_skinny_") + types[(i - kSkinny) / 8] + "_" + std::to_string(v / 2 + 1) + "x" + std::to_string(v % 2 + 1);
+    const int v = (i - kSkinny) % 4;
+    return std::string("kcg_mm8_skinny_") + types[(i - kSkinny) / 4] + "_" + std::to_string(v / 2 + 1) + "x" + std::to_string(v % 2 + 1);
   }
-  if (i < kMoeUp) return std::string("kcg_mm8_tile_") + tile[i - kTile];
+  if (i < kMoeUp) return std::string("kcg_mm8_tile_") + types[(i - kTile) / kTiles] + "_" + kTileTable[(i - kTile) % kTiles].name;
   if (i < kMoeDown) return std::string("kcg_moe_up_") + moe[i - kMoeUp];
   return std::string("kcg_moe_down_") + moe[(i - kMoeDown) / 2] + "_" + std::to_string((i - kMoeDown) % 2);
+}
+
+// What a product of these sizes (m, n > 0) with results of type t (0: bf16, 1: f16, 2: f32) runs.
+struct MatmulChoice {
+  int fn, threads, grid_m, grid_n;
+  int64_t blocks;
+};
+MatmulChoice choose_matmul(int64_t m, int64_t n, int64_t k, int t) {
+  const int64_t groups = (k + 127) / 128;
+  int rt = 0, tile = 0;                    // rt > 0: without a tile
+  if (m <= 16) {
+    rt = n >= 32 * 224 ? 2 : 1;            // 32 rows of b a block where that still fills the chip (8 x 8192 x 4096: 8.3 us, with 16 rows 9.5)
+  } else {
+    double best = 1e30;
+    for (int v = 0; v < kTiles - (t == 2); ++v) {
+      const double e = tile_estimate(kTileTable[v], m, n, groups);
+      if (e < best) {
+        best = e;
+        tile = v;
+      }
+    }
+    if (m <= 32)
+      for (int r = 1; r <= 2; ++r) {
+        const double e = skinny_estimate(r, n, groups);
+        if (e < best) {
+          best = e;
+          rt = r;
+        }
+      }
+  }
+  if (rt) return {kSkinny + t * 4 + (int)(m - 1) / 16 * 2 + rt - 1, SKINNY_WAVES * 64, 0, 0, (n + 16 * rt - 1) / (16 * rt)};
+  const Tile& v = kTileTable[tile];
+  const int64_t gm = (m + v.bm - 1) / v.bm, gn = (n + v.bn - 1) / v.bn;
+  return {kTile + t * kTiles + tile, v.threads, (int)gm, (int)gn, gm * gn};
 }
 
 struct DeviceKernels {
@@ -82,6 +150,7 @@ int kernels_on(const HostHip* hip, int device, const DeviceKernels** out) {
     hipError_t e = hip->ModuleLoadData(&k->module, kcg_ops_code);
     if (e != hipSuccess) return host_hip_fail(e, "hipModuleLoadData (operators)");
     for (int i = 0; i < kNumKernels && e == hipSuccess; ++i) {
+      if (i == kTile + 3 * kTiles - 1) continue;       // the largest tile has no form with float32 results
       e = hip->ModuleGetFunction(&k->fn[i], k->module, kernel_symbol(i).c_str());
       // a block of the experts' second kernel may use more than 64 KiB of LDS, part of it dynamic
       if (e == hipSuccess && i >= kMoeDown)
@@ -231,34 +300,29 @@ int kcg_matmul_fp8(const kcg_matmul_fp8_args* p, int device, uint64_t stream) {
     return bad("matmul_fp8: a stride of the scales is negative");
   // a tile addresses its rows with 32-bit offsets from its first one
   if ((p->m > 1 && p->a_stride > (1 << 22)) || (p->n > 1 && p->b_stride > (1 << 22)) || (p->m > 1 && p->a_scale_stride_row > (1 << 20)) ||
-      (p->n > 128 && p->b_scale_stride_row > (1 << 24)) || (p->k > 128 && p->b_scale_stride_group > (1 << 24)))
-    return bad("matmul_fp8: rows of a or b are more than 2^22 elements apart, of a_scale more than 2^20, or scales of b more than 2^24");
+      (p->n > 128 && p->b_scale_stride_row > (1 << 22)) || (p->k > 128 && (p->a_scale_stride_group > (1 << 22) || p->b_scale_stride_group > (1 << 22))))
+    return bad("matmul_fp8: rows of a or b, or scales, are more than 2^22 elements apart, or rows of a_scale more than 2^20");
   MatmulArgs a = {(const uint8_t*)p->a, (const uint8_t*)p->b, (const float*)p->a_scale, (const float*)p->b_scale, (void*)p->c,
                   p->m > 1 ? p->a_stride : 0, p->n > 1 ? p->b_stride : 0, p->c_stride, p->m > 1 ? p->a_scale_stride_row : 0, p->a_scale_stride_group,
                   p->b_scale_stride_row, p->b_scale_stride_group, (int)p->m, (int)p->n, (int)p->k, (int)groups(p->k), 0, 0, 0};
   a.c_wide = aligned(p->c, 4 * es) && (p->m == 1 || aligned(p->c_stride, 4));
-  int fn, block;
-  int64_t blocks;
-  if (p->m <= 64) {
-    // 32 rows of b a block where that still fills the chip: 37 x 8192 x 4096 takes 12.5 us so, 18.8 with 16 rows
-    const int rt = p->n >= 32 * 224 ? 2 : 1;
-    fn = kSkinny + t * 8 + (int)(p->m - 1) / 16 * 2 + rt - 1;
-    block = SKINNY_WAVES * 64;
-    blocks = (p->n + 16 * rt - 1) / (16 * rt);
-  } else {
-    static const int edge[3] = {256, 128, 64}, threads[3] = {512, 256, 256};
-    static const int first[3] = {kTile, kTile + 2, kTile + 5};
-    int v = t == 2 ? 1 : 0;                // (float32 results: the wide operands of a 256 x 256 tile do not fit the registers)
-    for (; v < 2; ++v)
-      if (((p->m + edge[v] - 1) / edge[v]) * ((p->n + edge[v] - 1) / edge[v]) >= 192) break;
-    a.grid_m = (int)((p->m + edge[v] - 1) / edge[v]);
-    a.grid_n = (int)((p->n + edge[v] - 1) / edge[v]);
-    blocks = (int64_t)a.grid_m * a.grid_n;
-    fn = first[v] + t;
-    block = threads[v];
+  const MatmulChoice c = choose_matmul(p->m, p->n, p->k, t);
+  if (c.blocks > (1 << 30)) return bad("matmul_fp8: m * n is too large");
+  a.grid_m = c.grid_m;
+  a.grid_n = c.grid_n;
+  return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) { return launch(hip, k.fn[c.fn], (unsigned)c.blocks, 1, c.threads, 0, stream, &a); });
+}
+
+int kcg_matmul_fp8_kernel(int64_t m, int64_t n, int64_t k, int64_t c_dtype, char* out, int out_len) {
+  const int t = type_index(c_dtype);
+  if (t < 0 || !extent_ok(m) || !extent_ok(n) || !extent_ok(k) || !out || out_len < 1) return bad("matmul_fp8_kernel: sizes in [0, 2^30], a 16 or 32-bit type, a buffer");
+  try {
+    const std::string s = m && n ? kernel_symbol(choose_matmul(m, n, k, t).fn) : "";
+    snprintf(out, (size_t)out_len, "%s", s.c_str());
+    return (int)s.size();
+  } catch (...) {
+    return KCG_ERR_ARGUMENT;
   }
-  if (blocks > (1 << 30)) return bad("matmul_fp8: m * n is too large");
-  return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) { return launch(hip, k.fn[fn], (unsigned)blocks, 1, block, 0, stream, &a); });
 }
 
 int64_t kcg_moe_workspace_bytes(int64_t tokens, int64_t experts, int64_t topk, int64_t hidden, int64_t inter) {

@@ -25,19 +25,23 @@ SWIGLU(float, f32)
     __shared__ f32x4 red[SKINNY_WAVES * CT * RT * 64];                                                         \
     skinny_kernel<TC, CT, RT, SKINNY_WAVES>(a, red);                                                           \
   }
-#define SKINNIES(TC, NAME) \
-  SKINNY(TC, NAME, 1, 1) SKINNY(TC, NAME, 1, 2) SKINNY(TC, NAME, 2, 1) SKINNY(TC, NAME, 2, 2) SKINNY(TC, NAME, 3, 1) SKINNY(TC, NAME, 3, 2) SKINNY(TC, NAME, 4, 1) SKINNY(TC, NAME, 4, 2)
-#define TILE(TC, NAME, BM, BN, WM, WN, S, WPE)                                                                         \
-  extern "C" __global__ void __launch_bounds__(WM * WN * 64, WPE) kcg_mm8_tile_##NAME##_##BM##x##BN(MatmulArgs a) {     \
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[TilePlan<BM, BN, WM, WN, S>::LDS];                          \
-    tile_kernel<TC, BM, BN, WM, WN, S>(a, smem);                                                                       \
+#define SKINNIES(TC, NAME) SKINNY(TC, NAME, 1, 1) SKINNY(TC, NAME, 1, 2) SKINNY(TC, NAME, 2, 1) SKINNY(TC, NAME, 2, 2)
+// BM x BN tile, WM x WN waves a group, S stages, KS groups; W: waves per SIMD the registers have to leave room for
+#define TILE(TC, NAME, BM, BN, WM, WN, S, KS, W)                                                                              \
+  extern "C" __global__ void __launch_bounds__(WM * WN * KS * 64, W) kcg_mm8_tile_##NAME##_##BM##x##BN##_##WM##x##WN##x##KS(   \
+      MatmulArgs a) {                                                                                                         \
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[TilePlan<BM, BN, WM, WN, S, KS>::LDS];                             \
+    tile_kernel<TC, BM, BN, WM, WN, S, KS>(a, smem);                                                                          \
   }
-#define MATMULS(TC, NAME) SKINNIES(TC, NAME) TILE(TC, NAME, 128, 128, 2, 2, 2, 2) TILE(TC, NAME, 64, 64, 2, 2, 4, 2)
+#define MATMULS(TC, NAME)                                                                                                     \
+  SKINNIES(TC, NAME)                                                                                                          \
+  TILE(TC, NAME, 32, 32, 2, 1, 4, 4, 2) TILE(TC, NAME, 64, 32, 4, 1, 4, 2, 2) TILE(TC, NAME, 64, 64, 2, 2, 4, 1, 2)           \
+  TILE(TC, NAME, 64, 64, 2, 2, 4, 2, 2) TILE(TC, NAME, 128, 128, 4, 2, 4, 1, 2) TILE(TC, NAME, 128, 128, 2, 2, 2, 1, 2)
 MATMULS(__bf16, bf16)
 MATMULS(_Float16, f16)
 MATMULS(float, f32)
-TILE(__bf16, bf16, 256, 256, 4, 2, 2, 2)
-TILE(_Float16, f16, 256, 256, 4, 2, 2, 2)
+TILE(__bf16, bf16, 256, 256, 4, 2, 2, 1, 2)
+TILE(_Float16, f16, 256, 256, 4, 2, 2, 1, 2)
 
 #define MOE(OPS, W, X, NAME)                                                                                        \
   extern "C" __global__ void __launch_bounds__(UP_WAVES * 64, 4) kcg_moe_up_##NAME(MoeArgs a) { up_kernel<OPS, W, X>(a); } \

@@ -108,12 +108,14 @@ __device__ void skinny_kernel(const MatmulArgs& p, f32x4* red) {
 // fragments are in registers by then: with S = 2 a fetch has most of a step to land, with more stages S - 1 steps; the
 // fragment reads of the next step run under the last row's matrix instructions, and the fma of a product under the next
 // two products.
+// KS > 1: KS groups of WM x WN waves take the steps in turn, each with stages of its own, and their sums meet in LDS.  A step
+// of a small tile is a chain of waits (0.28 us, whatever the number of tiles): this shortens the chain where tiles are few.
 // Scales come the same way in chunks of 8 steps, a chunk ahead: read per lane and step where they are needed, from rows
 // of their own, they made 4096^3 take 88 us, with rows side by side 70.
 // ---------------------------------------------------------------------------------------------
-template <int BM, int BN, int WM, int WN, int S>
+template <int BM, int BN, int WM, int WN, int S, int KS>
 struct TilePlan {
-  static constexpr int NT = WM * WN * 64;
+  static constexpr int NT = WM * WN * 64;          // threads of a group
   static constexpr int MB = BM / WM / 16, NB = BN / WN / 16;
   static constexpr int ROWS = BM + BN, STAGE = ROWS * GROUP;
   static constexpr int FETCH = ROWS * 8 / NT;      // 16-byte chunks a thread fetches for a stage
@@ -126,11 +128,12 @@ struct TilePlan {
   static constexpr int SB = BN >= GROUP ? BN / GROUP : 1;              // blocks of 128 rows of B a tile has scales from
   static constexpr int STEPS = 8;                                      // of a chunk of scales
   static constexpr int SCALES = STEPS * BM + 64;                       // floats of one: [step][row], then [block][step]
-  static constexpr int LDS = S * STAGE + 2 * SCALES * 4;
+  static constexpr int PART = S * STAGE + 2 * SCALES * 4, LDS = KS * PART;
+  static_assert((KS - 1) * BM * BN * 4 <= LDS, "the groups' sums");
   static_assert(BM % RPF == 0 && BN % RPF == 0 && NB >= 2 && NB % 2 == 0 && (S & (S - 1)) == 0 && SB * STEPS <= 64, "tile plan");
   static_assert(BN / WN <= GROUP && GROUP % (BN / WN) == 0, "a wave's rows of B lie in one block of 128");
   static_assert(S == 2 || LAST == FETCH, "the waits count whole fetches");
-  static_assert(BM % 64 == 0 && STEPS * BM / 64 % (NT / 64) == 0, "scales: whole waves");
+  static_assert((BM % 64 == 0 || 64 % BM == 0) && STEPS * BM / 64 % (NT / 64) == 0, "scales: whole waves");
 };
 
 // 16 (4) bytes a lane from base + off into consecutive LDS from lds on.  In assembly, because the compiler would wait for every
@@ -143,14 +146,16 @@ __device__ __forceinline__ void fetch_lds4(const void* base, unsigned off, unsig
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 
-template <class TC, int BM, int BN, int WM, int WN, int S>
-__device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
-  typedef TilePlan<BM, BN, WM, WN, S> P;
+template <class TC, int BM, int BN, int WM, int WN, int S, int KS>
+__device__ void tile_kernel(const MatmulArgs& p, uint8_t* lds) {
+  typedef TilePlan<BM, BN, WM, WN, S, KS> P;
   typedef typename DotOf<TC>::type Dot;
   constexpr int MB = P::MB, NB = P::NB, NW = WM * WN;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = KS > 1 ? wave_id / NW : 0, wave = wave_id - kg * NW, tid = wave * 64 + lane;     // group, and place in it
   const int wm = wave % WM, wn = wave / WM;
   const int r = lane & 15, g = lane >> 4;
+  uint8_t* const smem = lds + kg * P::PART;
 
   // block -> tile: ids are dealt round-robin to the 8 XCDs; each gets one contiguous part of the order, which walks the
   // n tiles of 4 tile rows together, so that an XCD's resident tiles share panels of both operands in its L2
@@ -165,7 +170,9 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
   const int gm = min(GM, p.grid_m - grp * GM);
   const int tm = grp * GM + in % gm, tn = in / gm;
   const int m0 = tm * BM, n0 = tn * BN;
-  const int KB = p.KB;
+  // step t of this group is group kb(t) of K; it has `steps` of them, every group at least p.KB / KS
+  const int steps = (p.KB - kg + KS - 1) / KS, last_step = (p.KB - 1) / KS;
+  auto group_of = [&](int t) { return t * KS + kg; };
 
   // fetch: thread -> row tid / 8 (+ RPF per further piece), place tid % 8
   const int frow = tid >> 3, fchunk = (tid & 7) ^ (frow & 7);     // (RPF is a multiple of 8: the swizzle is the same in every piece)
@@ -182,9 +189,10 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
   // a chunk of the partial last group that lies behind K: the row's first chunk of that group instead (cleared in LDS later)
   const bool ragged = (p.K & (GROUP - 1)) != 0;
   const bool behind = ragged && fchunk * 16 >= (p.K & (GROUP - 1));
-  auto fetch = [&](auto from_c, auto to_c, int kb) {       // pieces [from, to) of FETCH
-    const unsigned back = behind && kb == KB - 1 ? fchunk * 16 : 0;
-    const unsigned to = lds_wave + (kb & (S - 1)) * P::STAGE;
+  auto fetch = [&](auto from_c, auto to_c, int t) {        // pieces [from, to) of FETCH
+    const int kb = group_of(t);
+    const unsigned back = behind && kb == p.KB - 1 ? fchunk * 16 : 0;
+    const unsigned to = lds_wave + (t & (S - 1)) * P::STAGE;
     const uint8_t* ak = abase + (int64_t)kb * GROUP;
     const uint8_t* bk = bbase + (int64_t)kb * GROUP;
     static_for<decltype(from_c)::value, decltype(to_c)::value>([&](auto f_c) {
@@ -193,9 +201,10 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
     });
   };
   // zeros behind K in the stage of the partial last group
-  auto clear_tail = [&](int kb) {
+  auto clear_tail = [&](int t) {
+    if (group_of(t) != p.KB - 1) return;
     const int kt = p.K & (GROUP - 1);
-    uint8_t* st = smem + (kb & (S - 1)) * P::STAGE;
+    uint8_t* st = smem + (t & (S - 1)) * P::STAGE;
     for (int i = tid; i < P::ROWS * 8; i += P::NT) {
       const int row = i >> 3, c = i & 7;
       u32x4_a* at = (u32x4_a*)(st + row * GROUP + ((c ^ (row & 7)) << 4));
@@ -215,32 +224,34 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
   const unsigned sw0 = ((g ^ (r & 7)) << 4), sw1 = (((g + 4) ^ (r & 7)) << 4);
   const uint8_t* arow = smem + (wm * MB * 16 + r) * GROUP;
   const uint8_t* brow = smem + (BM + wn * NB * 16 + r) * GROUP;
-  auto frag = [&](const uint8_t* base, int i, int kb) {
-    const uint8_t* q = base + (kb & (S - 1)) * P::STAGE + i * 16 * GROUP;
+  auto frag = [&](const uint8_t* base, int i, int t) {
+    const uint8_t* q = base + (t & (S - 1)) * P::STAGE + i * 16 * GROUP;
     return join(*(const u32x4_a*)(q + sw0), *(const u32x4_a*)(q + sw1));
   };
-  // scales of chunk c (steps 8 c .. 8 c + 7): an instruction fetches 64 rows of one step, the last one those of the weights
-  constexpr int STEPS = P::STEPS, PARTS = BM / 64;
+  // scales of chunk c (the group's steps 8 c .. 8 c + 7): an instruction fetches 64 rows of one step, the last one those of the weights
+  constexpr int STEPS = P::STEPS;
   const float* const scales = (const float*)(smem + S * P::STAGE);
+  const unsigned sa_step = (unsigned)p.sa_k * KS, sb_step = (unsigned)p.sb_k * KS;
   auto fetch_scales = [&](int c) {
     const unsigned to = lds0 + S * P::STAGE + (c & 1) * P::SCALES * 4;
+    const int most = steps - 1 - c * STEPS;
+    const float* base = p.sa + (int64_t)m0 * p.sa_m + (int64_t)group_of(c * STEPS) * p.sa_k;
 #pragma unroll
-    for (int i = 0; i < STEPS * PARTS / NW; ++i) {
-      const int at = wave + i * NW, step = at / PARTS, part = at % PARTS;
-      const float* base = p.sa + (int64_t)m0 * p.sa_m + (int64_t)min(c * STEPS + step, KB - 1) * p.sa_k;
-      fetch_lds4(base, (unsigned)min(part * 64 + lane, p.M - 1 - m0) * (unsigned)p.sa_m * 4u, to + at * 256);
+    for (int i = 0; i < STEPS * BM / 64 / NW; ++i) {
+      const int at = (wave + i * NW) * 64 + lane, step = min(at / BM, most), row = min(at % BM, p.M - 1 - m0);
+      fetch_lds4(base, ((unsigned)row * (unsigned)p.sa_m + (unsigned)step * sa_step) * 4u, to + (wave + i * NW) * 256);
     }
     if (wave == 0) {
-      const float* base = p.sb + (int64_t)(n0 / GROUP) * p.sb_n + (int64_t)c * STEPS * p.sb_k;
-      const int block = min(min(lane / STEPS, P::SB - 1), (p.N - 1) / GROUP - n0 / GROUP), step = min(lane % STEPS, KB - 1 - c * STEPS);
-      fetch_lds4(base, (unsigned)block * (unsigned)p.sb_n * 4u + (unsigned)step * (unsigned)p.sb_k * 4u, to + STEPS * BM * 4);
+      const float* sb = p.sb + (int64_t)(n0 / GROUP) * p.sb_n + (int64_t)group_of(c * STEPS) * p.sb_k;
+      const int block = min(min(lane / STEPS, P::SB - 1), (p.N - 1) / GROUP - n0 / GROUP), step = min(lane % STEPS, most);
+      fetch_lds4(sb, ((unsigned)block * (unsigned)p.sb_n + (unsigned)step * sb_step) * 4u, to + STEPS * BM * 4);
     }
   };
   const float* my_sa = scales + wm * MB * 16 + r;
   const float* my_sb = scales + STEPS * BM + (n0 % GROUP + wn * NB * 16) / GROUP * STEPS;
   float s[MB], s_next[MB], sb_next;
-  auto read_scales = [&](float (&v)[MB], int kb) {
-    const int chunk = ((kb / STEPS) & 1) * P::SCALES, step = kb % STEPS;
+  auto read_scales = [&](float (&v)[MB], int t) {
+    const int chunk = ((t / STEPS) & 1) * P::SCALES, step = t % STEPS;
 #pragma unroll
     for (int j = 0; j < MB; ++j) v[j] = my_sa[chunk + step * BM + j * 16];
     sb_next = my_sb[chunk + step];
@@ -252,26 +263,29 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
 #pragma unroll
     for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  if (KB > 0) {
-    fetch_scales(0);
-    static_for<0, S - 1>([&](auto k_c) {
-      constexpr int k = decltype(k_c)::value;
-      if (k < KB) fetch(Int<0>(), Int<P::FETCH>(), k);
-    });
+  if (p.KB > 0) {
+    if (steps > 0) {
+      fetch_scales(0);
+      static_for<0, S - 1>([&](auto t_c) {
+        constexpr int t = decltype(t_c)::value;
+        if (t < steps) fetch(Int<0>(), Int<P::FETCH>(), t);
+      });
+    }
     // (in order: the first stage and the scales in front of it have landed when no more than the other stages are left)
-    if (KB >= S - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * P::FETCH) : "memory");
+    if (steps >= S - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * P::FETCH) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    read_scales(s, 0);
-#pragma unroll
-    for (int j = 0; j < MB; ++j) s[j] *= sb_next;
-    if (ragged && KB == 1) {
+    if (ragged && last_step == 0) {
       clear_tail(0);
       __syncthreads();
     }
-    if (S - 1 < KB) fetch(Int<0>(), Int<P::LAST>(), S - 1);
+    if (S - 1 < steps) fetch(Int<0>(), Int<P::LAST>(), S - 1);
     i32x8 am[MB], bn[4];                         // weight row i in place i % 4, two rows ahead of its products
+    // (a group without a step reads what lies there, and uses none of it)
+    read_scales(s, 0);
+#pragma unroll
+    for (int j = 0; j < MB; ++j) s[j] *= sb_next;
 #pragma unroll
     for (int j = 0; j < MB; ++j) am[j] = frag(arow, j, 0);
     bn[0] = frag(brow, 0, 0);
@@ -286,41 +300,40 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
       // (here, not behind the branches at the end of the step, where the compiler would gather them and keep every d until then)
       asm volatile("" : "+v"(acc[i][j]));
     };
-
-    for (int kb = 0; kb < KB; ++kb) {
-      const int nx = min(kb + 1, KB - 1);
+    auto step = [&](int t) {
+      const int nx = min(t + 1, steps - 1);
       typename Dot::frag af[MB];
 #pragma unroll
       for (int j = 0; j < MB; ++j) af[j] = Dot::make(am[j]);
       // (behind the stages fetched so far, in front of the ones to come: the waits below cover them)
-      if (kb % STEPS == 1 && kb - 1 + STEPS < KB) fetch_scales(kb / STEPS + 1);
+      if (t % STEPS == 1 && t - 1 + STEPS < steps) fetch_scales(t / STEPS + 1);
       static_for<0, NB>([&](auto i_c) {
         constexpr int i = decltype(i_c)::value;
         if constexpr (i == NB - 1) {
           // every fragment of this stage is in registers or on its way; the next stage has landed when no more than the S - 2
           // behind it are left
-          if (S > 2 && kb + S - 1 < KB) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * P::FETCH) : "memory");
+          if (S > 2 && t + S - 1 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * P::FETCH) : "memory");
           else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
           read_scales(s_next, nx);
-          if (ragged && kb + 1 == KB - 1) {
-            clear_tail(kb + 1);
+          if (ragged && t + 1 == last_step) {
+            clear_tail(t + 1);
             __syncthreads();
           }
-          if (kb + S < KB) fetch(Int<0>(), Int<P::LAST>(), kb + S);
+          if (t + S < steps) fetch(Int<0>(), Int<P::LAST>(), t + S);
         } else if constexpr (P::LAST + i * P::PER_ROW < P::FETCH) {
           constexpr int to = P::LAST + (i + 1) * P::PER_ROW;
-          if (kb + S - 1 < KB) fetch(Int<P::LAST + i * P::PER_ROW>(), Int<(to < P::FETCH ? to : P::FETCH)>(), kb + S - 1);
+          if (t + S - 1 < steps) fetch(Int<P::LAST + i * P::PER_ROW>(), Int<(to < P::FETCH ? to : P::FETCH)>(), t + S - 1);
         }
-        if constexpr (i + 2 < NB) bn[(i + 2) % 4] = frag(brow, i + 2, kb);
+        if constexpr (i + 2 < NB) bn[(i + 2) % 4] = frag(brow, i + 2, t);
         const typename Dot::frag bf = Dot::make(bn[i % 4]);
         static_for<0, MB>([&](auto j_c) {
           constexpr int j = decltype(j_c)::value, q = i * MB + j;
           d[q % 3] = Dot::mma(bf, af[j]);
           if constexpr (i == NB - 1) am[j] = frag(arow, j, nx);          // (after the last step: the same stage again, unused)
           if constexpr (i == NB - 1 && j == 0) bn[0] = frag(brow, 0, nx);
-          if constexpr (i == NB - 1 && j == (NB > 2 ? 1 : MB - 1)) bn[1] = frag(brow, 1, nx);   // (NB = 2: row 1 is this row)
+          if constexpr (i == NB - 1 && j == (NB > 2 && MB > 1 ? 1 : MB - 1)) bn[1] = frag(brow, 1, nx);   // (NB = 2: row 1 is this row)
           if constexpr (q >= 2) add(Int<q - 2>());
           __builtin_amdgcn_sched_barrier(0);
         });
@@ -329,8 +342,35 @@ __device__ void tile_kernel(const MatmulArgs& p, uint8_t* smem) {
       add(Int<NB * MB - 1>());
 #pragma unroll
       for (int j = 0; j < MB; ++j) s[j] = s_next[j] * sb_next;
+    };
+    // the steps that every group has, then those that only some have: the others keep them company at the barrier
+    const int common = p.KB / KS;
+    for (int t = 0; t < common; ++t) step(t);
+    if constexpr (KS > 1) {
+      if (common * KS < p.KB) {
+        if (common < steps) step(common);
+        else __builtin_amdgcn_s_barrier();
+      }
+      // sums of groups 1 .. KS - 1, in LDS behind the last reads of it, added by group 0 in their order
+      __syncthreads();
+      f32x4* sums = (f32x4*)lds;
+      if (kg > 0) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int j = 0; j < MB; ++j) sums[(((kg - 1) * NW + wave) * NB * MB + i * MB + j) * 64 + lane] = acc[i][j];
+      }
+      __syncthreads();
+      if (kg > 0) return;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < MB; ++j)
+#pragma unroll
+          for (int o = 0; o < KS - 1; ++o) acc[i][j] += sums[((o * NW + wave) * NB * MB + i * MB + j) * 64 + lane];
     }
   }
+  if (KS > 1 && kg > 0) return;
 #pragma unroll
   for (int j = 0; j < MB; ++j) {
     const int m = m0 + (wm * MB + j) * 16 + r;

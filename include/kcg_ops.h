@@ -73,6 +73,9 @@ typedef struct kcg_matmul_fp8_args {
   int64_t m, n, k, c_dtype;
 } kcg_matmul_fp8_args;
 int kcg_matmul_fp8(const kcg_matmul_fp8_args* args, int device, uint64_t stream);
+/* Name of the kernel that a product of these sizes runs (as a profiler shows it; "" for an empty one); needs no GPU.  Writes
+ * at most out_len bytes with the closing 0 and returns the name's length, or a negative status. */
+int kcg_matmul_fp8_kernel(int64_t m, int64_t n, int64_t k, int64_t c_dtype, char* out, int out_len);
 
 /* A layer of routed experts for at most 64 tokens: the topk largest logits of a token (equal ones: the lower index) choose
  * its experts, p = softmax over them (renormalize) or over all experts,

@@ -147,6 +147,29 @@ MATMULS = [(1, 1, 1, F32), (1, 16, 128, BF16), (2, 5, 15, F32), (3, 100, 127, F1
            (1, 512, 16384, F32), (256, 256, 4096, F32), (2100, 1500, 300, F32), (1800, 1790, 129, BF16), (3500, 3700, 200, F32), (4096, 4000, 640, F16), (3601, 3585, 127, BF16)]
 
 
+# sizes that between them run every kernel (tests/test_ops_cpu.py checks that), with whole and partial groups of K, fewer groups
+# than a tile's waves split into, and counts that the split does not divide
+KERNEL_SIZES = [(1, 200, 700), (16, 8000, 300), (20, 100, 500), (30, 7300, 500), (24, 300, 2900), (64, 500, 1301), (37, 8100, 1100), (60, 8192, 129), (200, 300, 100),
+                (500, 4000, 260), (250, 4000, 4230), (300, 3000, 2050), (1000, 4000, 1290), (2000, 4000, 700), (4000, 4050, 1290), (4096, 4096, 3000)]
+
+
+@pytest.mark.parametrize("m,n,k", KERNEL_SIZES)
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_matmul_kernels(m, n, k, out):
+    print(f"[case] matmul kernels {m}x{n}x{k} {out}", flush=True)
+    test_matmul(m, n, k, out)
+    # ... and with one value of NaN behind K in every row of both (the padding), whole numbers: exact in float32
+    g = gen(m + k)
+    a, b = (rows8(r, k, 0x7f)[1] for r in (m, n))
+    a.copy_(torch.randint(-2, 3, (m, k), device=DEV, generator=g).float().to(E4M3))
+    b.copy_(torch.randint(-2, 3, (n, k), device=DEV, generator=g).float().to(E4M3))
+    sa = 2.0 ** torch.randint(-1, 2, (m, R.groups(k)), device=DEV, generator=g).float()
+    sb = 2.0 ** torch.randint(-1, 2, (R.groups(n), R.groups(k)), device=DEV, generator=g).float()
+    want = R.widen(a, sa, False) @ R.widen(b, sb, True).t().contiguous()
+    assert 4 * 4 * 16 * k < 2 ** 24
+    assert torch.equal(matmul_fp8(a, sa, b, sb, out_dtype=out), want.to(out))
+
+
 @pytest.mark.parametrize("m,n,k,out", MATMULS)
 def test_matmul(m, n, k, out):
     print(f"[case] matmul {m}x{n}x{k} {out}", flush=True)
