@@ -28,30 +28,36 @@ using namespace kcg_ops;
 // ---- kernels ---------------------------------------------------------------------------------
 // The tiles of the 8-bit product (kcg_ops_matmul.h).  A call takes the one that this estimate of its time, in microseconds,
 // is smallest for: every round of blocks costs start + steps * step, where a round is one block on each of the 256 compute
-// units, or two where two fit one (step2: their step); steps = groups of 128 of K / ks.  Measured for 16-bit results at
-// N, K in {1024 .. 16384}; the estimates lie within 10 % of what was measured, some 20 % at the largest sizes.
+// units, or two where two fit one (step2: their step); steps = groups of 128 of K / ks.  Products with float32 results take
+// nearly twice the matrix instructions a step, so they have costs of their own.  Measured at N, K in {1024 .. 16384}; the
+// estimates lie within 10 % of what was measured, some 20 % at the largest sizes and between one round and two.
+struct Cost {
+  float start, step, step2;
+};
 struct Tile {
   const char* name;
   int bm, bn, ks, threads;
-  float start, step, step2;
+  Cost half, full;                                        // 16-bit results, float32 results
 };
 const Tile kTileTable[] = {
-    {"32x32_2x1x4", 32, 32, 4, 512, 1.6f, .39f, 0.f},       // 37 x 1024 x 4096: 6.9 us (64 x 64: 12.4)
-    {"64x32_4x1x2", 64, 32, 2, 512, 1.2f, .36f, 0.f},       // 37 x 8192 x 4096: 9.5 (32 x 32: 12.8, 64 x 64 by two: 10.8)
-    {"64x64_2x2x1", 64, 64, 1, 256, .4f, .305f, .52f},      // 512 x 4096 x 1024: 7.3 (by two: 10.8)
-    {"64x64_2x2x2", 64, 64, 2, 512, 1.9f, .43f, 0.f},       // 256 x 4096 x 4096: 11.3 (by one: 12.8)
-    {"128x128_4x2x1", 128, 128, 1, 512, 2.f, .575f, 0.f},   // 1024 x 4096 x 4096: 24.8 (4 waves: 28.1)
-    {"128x128_2x2x1", 128, 128, 1, 256, 1.6f, .655f, 1.1f}, // 2048 x 4096 x 4096: 39.2 (8 waves: 46.2)
-    {"256x256_4x2x1", 256, 256, 1, 512, 7.f, 1.55f, 0.f},   // 4096^3: 63.0 (128 x 128: 75.1); 16-bit results
+    {"32x32_2x1x4", 32, 32, 4, 512, {1.6f, .39f, 0.f}, {1.9f, .64f, 0.f}},        // 37 x 4096 x 4096: 7.4 us (64 x 64: 12.4)
+    {"64x32_4x1x2", 64, 32, 2, 512, {1.2f, .36f, 0.f}, {1.4f, .62f, 0.f}},        // 37 x 8192 x 4096: 9.5 (32 x 32: 12.8, 64 x 64 by two: 10.8)
+    {"64x64_2x2x1", 64, 64, 1, 256, {.4f, .305f, .52f}, {1.2f, .52f, .74f}},      // 512 x 4096 x 1024: 7.2 (by two: 10.8)
+    {"64x64_2x2x2", 64, 64, 2, 512, {1.9f, .43f, 0.f}, {2.2f, .76f, 0.f}},        // 256 x 4096 x 4096: 11.3 (by one: 12.8)
+    {"64x128_2x2x1", 64, 128, 1, 256, {.8f, .6f, .67f}, {1.6f, .74f, 1.07f}},     // 4096 x 1536 x 1000, float32: 22.4 (64 x 64: 28.1, 128 x 128: 25.0)
+    {"128x128_2x2x1", 128, 128, 1, 256, {1.6f, .655f, 1.1f}, {4.6f, 1.08f, 1.75f}},  // 2048 x 4096 x 4096: 39.2 (8 waves: 46.2)
+    // for 16-bit results only: the next is no faster than 64 x 128 with float32 ones, the last has no registers for them
+    {"128x128_4x2x1", 128, 128, 1, 512, {2.f, .575f, 0.f}, {}},                   // 1024 x 4096 x 4096: 24.8 (4 waves: 28.1)
+    {"256x256_4x2x1", 256, 256, 1, 512, {7.f, 1.55f, 0.f}, {}},                   // 4096^3: 63.0 (128 x 128: 75.1)
 };
-constexpr int kTiles = sizeof(kTileTable) / sizeof(kTileTable[0]);
+constexpr int kTiles = sizeof(kTileTable) / sizeof(kTileTable[0]), kTilesF32 = kTiles - 2;
 constexpr double kLaunch = 2.3;
 
-double tile_estimate(const Tile& v, int64_t m, int64_t n, int64_t groups) {
+double tile_estimate(const Tile& v, const Cost& c, int64_t m, int64_t n, int64_t groups) {
   const double tiles = (double)((m + v.bm - 1) / v.bm) * (double)((n + v.bn - 1) / v.bn), steps = (double)((groups + v.ks - 1) / v.ks);
-  if (v.step2 == 0.f) return kLaunch + std::ceil(tiles / 256) * (v.start + steps * v.step);
+  if (c.step2 == 0.f) return kLaunch + std::ceil(tiles / 256) * (c.start + steps * c.step);
   const double full = std::floor(tiles / 512), rest = tiles - 512 * full;
-  return kLaunch + full * (v.start + steps * v.step2) + (rest > 0 ? v.start + steps * (rest <= 256 ? v.step : v.step2) : 0);
+  return kLaunch + full * (c.start + steps * c.step2) + (rest > 0 ? c.start + steps * (rest <= 256 ? c.step : c.step2) : 0);
 }
 // 17 to 32 rows without a tile (rt: 16-row tiles of b a block): N / 16 / rt blocks
 double skinny_estimate(int rt, int64_t n, int64_t groups) {
@@ -88,8 +94,8 @@ MatmulChoice choose_matmul(int64_t m, int64_t n, int64_t k, int t) {
     rt = n >= 32 * 224 ? 2 : 1;            // 32 rows of b a block where that still fills the chip (8 x 8192 x 4096: 8.3 us, with 16 rows 9.5)
   } else {
     double best = 1e30;
-    for (int v = 0; v < kTiles - (t == 2); ++v) {
-      const double e = tile_estimate(kTileTable[v], m, n, groups);
+    for (int v = 0; v < (t == 2 ? kTilesF32 : kTiles); ++v) {
+      const double e = tile_estimate(kTileTable[v], t == 2 ? kTileTable[v].full : kTileTable[v].half, m, n, groups);
       if (e < best) {
         best = e;
         tile = v;
@@ -150,7 +156,7 @@ int kernels_on(const HostHip* hip, int device, const DeviceKernels** out) {
     hipError_t e = hip->ModuleLoadData(&k->module, kcg_ops_code);
     if (e != hipSuccess) return host_hip_fail(e, "hipModuleLoadData (operators)");
     for (int i = 0; i < kNumKernels && e == hipSuccess; ++i) {
-      if (i == kTile + 3 * kTiles - 1) continue;       // the largest tile has no form with float32 results
+      if (i >= kTile + 2 * kTiles + kTilesF32 && i < kMoeUp) continue;       // tiles without a form for float32 results
       e = hip->ModuleGetFunction(&k->fn[i], k->module, kernel_symbol(i).c_str());
       // a block of the experts' second kernel may use more than 64 KiB of LDS, part of it dynamic
       if (e == hipSuccess && i >= kMoeDown)
