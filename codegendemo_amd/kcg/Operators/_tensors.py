@@ -29,33 +29,42 @@ def check(status):
 
 def matrix(name, t, rows, cols, dtype, device):
     """A [rows, cols] tensor of `dtype` on `device` whose rows are contiguous; returns its row stride."""
-    if t.dtype is not dtype or t.device != device:
-        raise TypeError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise ValueError(f"{name} must have shape ({rows}, {cols}), got {tuple(t.shape)}")
-    s = t.stride()
-    if s[1] != 1 and cols > 1:
+    if t.dtype is dtype and t.device == device and t.shape == (rows, cols):
+        s = t.stride()
+        if s[1] == 1 or cols <= 1:
+            return s[0]
         raise ValueError(f"{name}: the elements of a row must lie side by side, got strides {s}")
-    return s[0]
+    refuse(name, t, rows, cols, dtype, device)
 
 
 def strides2(name, t, rows, cols, device):
     """A float32 [rows, cols] tensor of any strides; returns them."""
-    if t.dtype is not torch.float32 or t.device != device:
-        raise TypeError(f"{name} must be torch.float32 on {device}, got {t.dtype} on {t.device}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise ValueError(f"{name} must have shape ({rows}, {cols}), got {tuple(t.shape)}")
-    return t.stride()
+    if t.dtype is torch.float32 and t.device == device and t.shape == (rows, cols):
+        return t.stride()
+    refuse(name, t, rows, cols, torch.float32, device)
+
+
+def refuse(name, t, rows, cols, dtype, device):
+    if t.dtype is not dtype or t.device != device:
+        raise TypeError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
+    raise ValueError(f"{name} must have shape ({rows}, {cols}), got {tuple(t.shape)}")
 
 
 def on_gpu(name, t):
     """The device of the tensor, which has to be a GPU; no operator has another path."""
-    d = t.device
-    if d.type != "cuda":
-        raise TypeError(f"{name} must be on a GPU, got {d}: the operators have no CPU path")
-    return d
+    if not t.is_cuda:
+        raise TypeError(f"{name} must be on a GPU, got {t.device}: the operators have no CPU path")
+    return t.device
 
 
-def empty_e4m3(rows, cols, device):
-    """An e4m3 matrix whose rows start on 16 bytes."""
-    return torch.empty((rows, -(-cols // 16) * 16), dtype=E4M3, device=device)[:, :cols]
+# Outputs an operator makes itself: known strides, so they pass by the checks.  A small call is over sooner on the GPU than
+# on the host, where making an output by torch.empty and slicing it would cost as much as all of the checks.
+
+def new_e4m3(rows, cols, device):
+    """An e4m3 matrix whose rows start on 16 bytes, and its row stride."""
+    ld = -(-cols // 16) * 16
+    return torch.empty_strided((rows, cols), (ld, 1), dtype=E4M3, device=device), ld
+
+
+def new_matrix(rows, cols, dtype, device):
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)

@@ -3,7 +3,7 @@ run-time arguments (a serving program's row count changes from call to call), so
 import torch
 
 from ... import _native_ops
-from ._tensors import CODE, E4M3, check, groups, matrix, on_gpu, stream_of, strides2
+from ._tensors import CODE, E4M3, check, groups, matrix, new_matrix, on_gpu, stream_of, strides2
 
 
 def matmul_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16):
@@ -20,14 +20,18 @@ def matmul_fp8(a, a_scale, b, b_scale, out=None, out_dtype=torch.bfloat16):
     (m, k), n = a.shape, b.shape[0]
     a_s = matrix("a", a, m, k, E4M3, device)
     b_s = matrix("b", b, n, k, E4M3, device)
-    as_m, as_g = strides2("a_scale", a_scale, m, groups(k), device)
-    bs_n, bs_g = strides2("b_scale", b_scale, groups(n), groups(k), device)
+    g = groups(k)
+    as_m, as_g = strides2("a_scale", a_scale, m, g, device)
+    bs_n, bs_g = strides2("b_scale", b_scale, groups(n), g, device)
+    if out is not None:
+        out_dtype = out.dtype
+    code = CODE.get(out_dtype)
+    if code is None or out_dtype is E4M3:
+        raise TypeError(f"out must be bfloat16, float16 or float32, got {out_dtype}")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype, device=device)
-    code = CODE.get(out.dtype)
-    if code is None or out.dtype is E4M3:
-        raise TypeError(f"out must be bfloat16, float16 or float32, got {out.dtype}")
-    o_s = matrix("out", out, m, n, out.dtype, device)
+        out, o_s = new_matrix(m, n, out_dtype, device), n
+    else:
+        o_s = matrix("out", out, m, n, out_dtype, device)
     if m and n:
         check(_native_ops.lib().kcg_matmul_fp8(
             _native_ops.MATMUL_FP8.pack(a.data_ptr(), a_scale.data_ptr(), b.data_ptr(), b_scale.data_ptr(), out.data_ptr(), a_s, as_m, as_g, b_s, bs_n,

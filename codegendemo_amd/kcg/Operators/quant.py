@@ -5,7 +5,7 @@ nearest even.  Both run on torch's current stream of the tensors' device; the fo
 import torch
 
 from ... import _native_ops
-from ._tensors import CODE, E4M3, check, empty_e4m3, groups, matrix, on_gpu, stream_of, strides2
+from ._tensors import CODE, E4M3, check, groups, matrix, new_e4m3, new_matrix, on_gpu, stream_of, strides2
 
 
 def rmsnorm_quant(x, weight, eps=1e-6, residual=None, residual_out=None, q=None, scale=None, y=None, want_y=False):
@@ -32,22 +32,27 @@ def rmsnorm_quant(x, weight, eps=1e-6, residual=None, residual_out=None, q=None,
     if residual is not None:
         r_s = matrix("residual", residual, t, h, dtype, device)
         if residual_out is None:
-            residual_out = torch.empty((t, h), dtype=dtype, device=device)
-        ro_s = matrix("residual_out", residual_out, t, h, dtype, device)
+            residual_out, ro_s = new_matrix(t, h, dtype, device), h
+        else:
+            ro_s = matrix("residual_out", residual_out, t, h, dtype, device)
         r_p, ro_p = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out without a residual")
     if q is None:
-        q = empty_e4m3(t, h, device)
-    q_s = matrix("q", q, t, h, E4M3, device)
+        q, q_s = new_e4m3(t, h, device)
+    else:
+        q_s = matrix("q", q, t, h, E4M3, device)
+    s_t, s_g = groups(h), 1
     if scale is None:
-        scale = torch.empty((t, groups(h)), dtype=torch.float32, device=device)
-    s_t, s_g = strides2("scale", scale, t, groups(h), device)
-    if y is None and want_y:
-        y = torch.empty((t, h), dtype=dtype, device=device)
+        scale = new_matrix(t, s_t, torch.float32, device)
+    else:
+        s_t, s_g = strides2("scale", scale, t, s_t, device)
     y_p = y_s = 0
     if y is not None:
         y_p, y_s = y.data_ptr(), matrix("y", y, t, h, dtype, device)
+    elif want_y:
+        y, y_s = new_matrix(t, h, dtype, device), h
+        y_p = y.data_ptr()
     code = CODE[dtype]
     if t and h:
         check(_native_ops.lib().kcg_rmsnorm_quant(
@@ -71,11 +76,14 @@ def swiglu_quant(gate_up, q=None, scale=None):
     t, i = gate_up.shape[0], gate_up.shape[1] // 2
     in_s = matrix("gate_up", gate_up, t, 2 * i, dtype, device)
     if q is None:
-        q = empty_e4m3(t, i, device)
-    q_s = matrix("q", q, t, i, E4M3, device)
+        q, q_s = new_e4m3(t, i, device)
+    else:
+        q_s = matrix("q", q, t, i, E4M3, device)
+    s_t, s_g = groups(i), 1
     if scale is None:
-        scale = torch.empty((t, groups(i)), dtype=torch.float32, device=device)
-    s_t, s_g = strides2("scale", scale, t, groups(i), device)
+        scale = new_matrix(t, s_t, torch.float32, device)
+    else:
+        s_t, s_g = strides2("scale", scale, t, s_t, device)
     if t and i:
         check(_native_ops.lib().kcg_swiglu_quant(
             _native_ops.SWIGLU_QUANT.pack(gate_up.data_ptr(), q.data_ptr(), scale.data_ptr(), in_s, q_s, s_t, s_g, t, i, CODE[dtype]),
