@@ -1,0 +1,277 @@
+// kcg_torch.cc — the small operators of the 8-bit path on torch tensors: checks of the arguments, outputs, the call.
+// A call of theirs is over in 3 to 5 us on the GPU, and the runtime's launch takes the host 3.1; with the same steps in Python a
+// call took the host 7.4 to 8.5 us (an output 1.3, a checked operand 0.5), so a decoded token waited for it.  Here a whole call
+// takes 4.3 to 4.7 us.
+//
+// The module links neither the library nor a HIP runtime: bind() gives it the addresses of the C entry points
+// (include/kcg_ops.h), so that both bindings run the one library that the process has loaded.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <ATen/ops/empty_strided.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include "../../include/kcg_gemm.h"
+#include "../../include/kcg_ops.h"
+
+namespace {
+
+using at::ScalarType;
+
+int (*norm_entry)(const kcg_rmsnorm_quant_args*, int, uint64_t);
+int (*swiglu_entry)(const kcg_swiglu_quant_args*, int, uint64_t);
+int (*matmul_entry)(const kcg_matmul_fp8_args*, int, uint64_t);
+PyObject* stream_of;       // device index -> raw handle of torch's current stream
+PyObject* check_status;    // raises what a negative status stands for
+
+int64_t groups(int64_t n) { return (n + 127) / 128; }
+int64_t address(const at::Tensor& t) { return (int64_t)(uintptr_t)t.data_ptr(); }
+
+int64_t code_of(ScalarType t) {
+  switch (t) {
+    case ScalarType::Float: return KCG_DT_FLOAT32;
+    case ScalarType::Half: return KCG_DT_FLOAT16;
+    case ScalarType::BFloat16: return KCG_DT_BFLOAT16;
+    default: return 0;     // no type of an input or a product here
+  }
+}
+
+const at::Tensor& tensor(const char* name, PyObject* o) {
+  TORCH_CHECK_TYPE(THPVariable_Check(o), name, " must be a tensor, got ", Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+
+void on_gpu(const char* name, const at::Tensor& t) {
+  TORCH_CHECK_TYPE(t.is_cuda(), name, " must be on a GPU, got ", t.device().str(), ": the operators have no CPU path");
+}
+
+void check_shape(const char* name, const at::Tensor& t, int64_t rows, int64_t cols, ScalarType type, at::Device device) {
+  TORCH_CHECK_TYPE(t.scalar_type() == type && t.device() == device, name, " must be ", c10::toString(type), " on ", device.str(), ", got ",
+                   c10::toString(t.scalar_type()), " on ", t.device().str());
+  TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, name, " must have shape (", rows, ", ", cols,
+                    "), got ", t.sizes());
+}
+
+// a matrix whose rows are contiguous -> its row stride
+int64_t matrix(const char* name, const at::Tensor& t, int64_t rows, int64_t cols, ScalarType type, at::Device device) {
+  check_shape(name, t, rows, cols, type, device);
+  TORCH_CHECK_VALUE(t.stride(1) == 1 || cols <= 1, name, ": the elements of a row must lie side by side, got strides ", t.strides());
+  return t.stride(0);
+}
+
+// What an argument stands for: the tensor given, checked, or a new one whose rows are `ld` apart.
+struct Matrix {
+  int64_t address = 0, row = 0, col = 0;
+  PyObject* object = nullptr;                // a new reference, or null
+  Matrix() = default;
+  Matrix(const Matrix&) = delete;
+  ~Matrix() { Py_XDECREF(object); }
+  PyObject* release() {
+    PyObject* o = object ? object : Py_NewRef(Py_None);
+    object = nullptr;
+    return o;
+  }
+  void made(int64_t rows, int64_t cols, int64_t ld, ScalarType type, at::Device device) {
+    at::Tensor t = at::empty_strided({rows, cols}, {ld, 1}, at::TensorOptions().dtype(type).device(device));
+    address = ::address(t);
+    row = ld;
+    col = 1;
+    object = THPVariable_Wrap(std::move(t));
+    if (!object) throw python_error();
+  }
+  void given(const char* name, PyObject* o, int64_t rows, int64_t cols, ScalarType type, at::Device device) {
+    const at::Tensor& t = tensor(name, o);
+    row = matrix(name, t, rows, cols, type, device);
+    col = 1;
+    address = ::address(t);
+    object = Py_NewRef(o);
+  }
+  void given_any_strides(const char* name, PyObject* o, int64_t rows, int64_t cols, at::Device device) {
+    const at::Tensor& t = tensor(name, o);
+    check_shape(name, t, rows, cols, ScalarType::Float, device);
+    row = t.stride(0);
+    col = t.stride(1);
+    address = ::address(t);
+    object = Py_NewRef(o);
+  }
+  void output(const char* name, PyObject* o, int64_t rows, int64_t cols, int64_t ld, ScalarType type, at::Device device) {
+    if (o == Py_None)
+      made(rows, cols, ld, type, device);
+    else
+      given(name, o, rows, cols, type, device);
+  }
+  void output_scales(PyObject* o, int64_t rows, int64_t cols, at::Device device) {
+    if (o == Py_None)
+      made(rows, cols, cols, ScalarType::Float, device);
+    else
+      given_any_strides("scale", o, rows, cols, device);
+  }
+};
+
+int64_t ld16(int64_t cols) { return (cols + 15) / 16 * 16; }
+
+// false: a Python error is set
+template <class Args>
+bool run(int (*entry)(const Args*, int, uint64_t), const Args& args, int device) {
+  PyObject* index = PyLong_FromLong(device);
+  PyObject* handle = index ? PyObject_CallOneArg(stream_of, index) : nullptr;
+  Py_XDECREF(index);
+  const uint64_t stream = handle ? PyLong_AsUnsignedLongLongMask(handle) : 0;
+  Py_XDECREF(handle);
+  if (!handle || PyErr_Occurred()) return false;
+  const int status = entry(&args, device, stream);
+  if (status >= 0) return true;
+  PyObject* r = PyObject_CallFunction(check_status, "i", status);      // raises
+  Py_XDECREF(r);
+  if (r) PyErr_Format(PyExc_RuntimeError, "status %d", status);
+  return false;
+}
+
+bool count(const char* name, Py_ssize_t n, Py_ssize_t want) {
+  if (n == want) return true;
+  PyErr_Format(PyExc_TypeError, "%s takes %zd arguments, got %zd", name, want, n);
+  return false;
+}
+
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!count("bind", n, 5)) return nullptr;
+  const uint64_t entries[3] = {PyLong_AsUnsignedLongLong(a[0]), PyLong_AsUnsignedLongLong(a[1]), PyLong_AsUnsignedLongLong(a[2])};
+  if (PyErr_Occurred()) return nullptr;
+  norm_entry = (decltype(norm_entry))(uintptr_t)entries[0];
+  swiglu_entry = (decltype(swiglu_entry))(uintptr_t)entries[1];
+  matmul_entry = (decltype(matmul_entry))(uintptr_t)entries[2];
+  Py_XDECREF(stream_of);
+  Py_XDECREF(check_status);
+  stream_of = Py_NewRef(a[3]);
+  check_status = Py_NewRef(a[4]);
+  Py_RETURN_NONE;
+}
+
+// (x, weight, eps, residual, residual_out, q, scale, y, want_y) -> (q, scale, y, residual_out)
+PyObject* rmsnorm_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!count("rmsnorm_quant", n, 9)) return nullptr;
+  const at::Tensor& x = tensor("x", a[0]);
+  on_gpu("x", x);
+  TORCH_CHECK_VALUE(x.dim() == 2, "x must be a matrix, got shape ", x.sizes());
+  const ScalarType type = x.scalar_type();
+  TORCH_CHECK_TYPE(code_of(type), "x must be bfloat16, float16 or float32, got ", c10::toString(type));
+  const at::Device device = x.device();
+  kcg_rmsnorm_quant_args p = {};
+  p.rows = x.size(0);
+  p.cols = x.size(1);
+  p.x_stride = matrix("x", x, p.rows, p.cols, type, device);
+  p.x = address(x);
+  p.dtype = code_of(type);
+  const at::Tensor& weight = tensor("weight", a[1]);
+  const ScalarType wt = weight.scalar_type();
+  TORCH_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == p.cols && (p.cols <= 1 || weight.stride(0) == 1) && weight.device() == device &&
+                        (wt == type || wt == ScalarType::Float),
+                    "weight must be a contiguous vector of ", p.cols, " values of ", c10::toString(type), " or Float on ", device.str());
+  p.weight = address(weight);
+  p.weight_dtype = code_of(wt);
+  p.eps = PyFloat_AsDouble(a[2]);
+  if (PyErr_Occurred()) return nullptr;
+  Matrix residual, residual_out, q, scale, y;
+  if (a[3] != Py_None) {
+    residual.given("residual", a[3], p.rows, p.cols, type, device);
+    residual_out.output("residual_out", a[4], p.rows, p.cols, p.cols, type, device);
+  } else {
+    TORCH_CHECK_VALUE(a[4] == Py_None, "residual_out without a residual");
+  }
+  q.output("q", a[5], p.rows, p.cols, ld16(p.cols), ScalarType::Float8_e4m3fn, device);
+  scale.output_scales(a[6], p.rows, groups(p.cols), device);
+  const int want_y = PyObject_IsTrue(a[8]);
+  if (want_y < 0) return nullptr;
+  if (want_y || a[7] != Py_None) y.output("y", a[7], p.rows, p.cols, p.cols, type, device);
+  p.residual = residual.address, p.residual_stride = residual.row;
+  p.residual_out = residual_out.address, p.residual_out_stride = residual_out.row;
+  p.q = q.address, p.q_stride = q.row;
+  p.scale = scale.address, p.scale_stride_row = scale.row, p.scale_stride_group = scale.col;
+  p.y = y.address, p.y_stride = y.row;
+  if (p.rows && p.cols && !run(norm_entry, p, device.index())) return nullptr;
+  PyObject* r = PyTuple_New(4);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, q.release());
+  PyTuple_SET_ITEM(r, 1, scale.release());
+  PyTuple_SET_ITEM(r, 2, y.release());
+  PyTuple_SET_ITEM(r, 3, residual_out.release());
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// (gate_up, q, scale) -> (q, scale)
+PyObject* swiglu_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!count("swiglu_quant", n, 3)) return nullptr;
+  const at::Tensor& gate_up = tensor("gate_up", a[0]);
+  on_gpu("gate_up", gate_up);
+  TORCH_CHECK_VALUE(gate_up.dim() == 2 && gate_up.size(1) % 2 == 0, "gate_up must be a matrix with an even number of columns, got shape ", gate_up.sizes());
+  const ScalarType type = gate_up.scalar_type();
+  TORCH_CHECK_TYPE(code_of(type), "gate_up must be bfloat16, float16 or float32, got ", c10::toString(type));
+  const at::Device device = gate_up.device();
+  kcg_swiglu_quant_args p = {};
+  p.rows = gate_up.size(0);
+  p.cols = gate_up.size(1) / 2;
+  p.gate_up_stride = matrix("gate_up", gate_up, p.rows, 2 * p.cols, type, device);
+  p.gate_up = address(gate_up);
+  p.dtype = code_of(type);
+  Matrix q, scale;
+  q.output("q", a[1], p.rows, p.cols, ld16(p.cols), ScalarType::Float8_e4m3fn, device);
+  scale.output_scales(a[2], p.rows, groups(p.cols), device);
+  p.q = q.address, p.q_stride = q.row;
+  p.scale = scale.address, p.scale_stride_row = scale.row, p.scale_stride_group = scale.col;
+  if (p.rows && p.cols && !run(swiglu_entry, p, device.index())) return nullptr;
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, q.release());
+  PyTuple_SET_ITEM(r, 1, scale.release());
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// (a, a_scale, b, b_scale, out, out_dtype) -> out
+PyObject* matmul_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!count("matmul_fp8", n, 6)) return nullptr;
+  const at::Tensor &ta = tensor("a", a[0]), &tb = tensor("b", a[2]);
+  on_gpu("a", ta);
+  TORCH_CHECK_VALUE(ta.dim() == 2 && tb.dim() == 2, "a and b must be matrices, got shapes ", ta.sizes(), " and ", tb.sizes());
+  const at::Device device = ta.device();
+  kcg_matmul_fp8_args p = {};
+  p.m = ta.size(0);
+  p.k = ta.size(1);
+  p.n = tb.size(0);
+  p.a_stride = matrix("a", ta, p.m, p.k, ScalarType::Float8_e4m3fn, device);
+  p.b_stride = matrix("b", tb, p.n, p.k, ScalarType::Float8_e4m3fn, device);
+  p.a = address(ta);
+  p.b = address(tb);
+  Matrix sa, sb, out;
+  sa.given_any_strides("a_scale", a[1], p.m, groups(p.k), device);
+  sb.given_any_strides("b_scale", a[3], groups(p.n), groups(p.k), device);
+  ScalarType type;
+  if (a[4] != Py_None) {
+    type = tensor("out", a[4]).scalar_type();
+  } else {
+    TORCH_CHECK_TYPE(THPDtype_Check(a[5]), "out_dtype must be a torch.dtype, got ", Py_TYPE(a[5])->tp_name);
+    type = reinterpret_cast<THPDtype*>(a[5])->scalar_type;
+  }
+  TORCH_CHECK_TYPE(code_of(type), "out must be bfloat16, float16 or float32, got ", c10::toString(type));
+  out.output("out", a[4], p.m, p.n, p.n, type, device);
+  p.c_dtype = code_of(type);
+  p.a_scale = sa.address, p.a_scale_stride_row = sa.row, p.a_scale_stride_group = sa.col;
+  p.b_scale = sb.address, p.b_scale_stride_row = sb.row, p.b_scale_stride_group = sb.col;
+  p.c = out.address, p.c_stride = out.row;
+  if (p.m && p.n && !run(matmul_entry, p, device.index())) return nullptr;
+  return out.release();
+  END_HANDLE_TH_ERRORS
+}
+
+#define METHOD(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {METHOD(bind), METHOD(rmsnorm_quant), METHOD(swiglu_quant), METHOD(matmul_fp8), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kcg_torch", "The small operators of the 8-bit path on torch tensors.", -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__kcg_torch(void) { return PyModule_Create(&module); }

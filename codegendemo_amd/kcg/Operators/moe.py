@@ -2,7 +2,7 @@
 import torch
 
 from ... import _native_ops
-from ._tensors import CODE, E4M3, check, groups, matrix, new_matrix, on_gpu, stream_of
+from ._tensors import CODE, E4M3, check, groups, matrix, on_gpu, stream_of
 
 MAX_TOKENS = 64
 
@@ -59,11 +59,10 @@ def moe_layer(x, logits, topk, w13, w2, w13_scale=None, w2_scale=None, renormali
         raise ValueError("bfloat16 weights have no scales")
     need = _native_ops.moe_workspace_bytes(t, e, topk, h, i)
     if out is None:
-        out, o_s = new_matrix(t, h, x.dtype, device), h
-    else:
-        o_s = matrix("out", out, t, h, x.dtype, device)
-    ids = new_matrix(t, topk, torch.int32, device)
-    probs = new_matrix(t, topk, torch.float32, device)
+        out = torch.empty((t, h), dtype=x.dtype, device=device)
+    o_s = matrix("out", out, t, h, x.dtype, device)
+    ids = torch.empty((t, topk), dtype=torch.int32, device=device)
+    probs = torch.empty((t, topk), dtype=torch.float32, device=device)
     if t:
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         check(_native_ops.lib().kcg_moe_layer(
