@@ -125,6 +125,19 @@ __device__ __forceinline__ u32x2 quantize_group(const float (&v)[8], float& scal
   return u32x2{(unsigned)lo, (unsigned)hi};
 }
 
+// g / (1 + exp(-g)) * up to 8 half steps of float32 while exp(-g) is in range, and g * 0 * up behind it (g < -87), in two
+// transcendental and nine other instructions; expf and a division take some thirty.  exp(-g) = 2^p (1 + lo ln 2), where lo is
+// what the rounding of p = -g log2(e) left out (times |g| otherwise, which is what expf reduces its argument against).
+// lo counts only where 2^p is neither 0 nor infinite; the maximum keeps the factor positive (and not NaN) elsewhere, so that
+// an infinite 2^p gives 0 and g = infinity gives infinity.  NaN stays NaN through p.
+__device__ __forceinline__ float silu_times(float g, float up) {
+  constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596299e-8f, LN2 = 0.693147182f;
+  const float p = g * -LOG2E;
+  const float lo = fmaf(g, -LOG2E_REST, fmaf(g, -LOG2E, -p));
+  const float den = fmaf(__builtin_amdgcn_exp2f(p), fmaxf(fmaf(lo, LN2, 1.f), .5f), 1.f);
+  return g * __builtin_amdgcn_rcpf(den) * up;
+}
+
 // 8 bytes of a quantised row whose start is 16-byte aligned; bytes behind the row's end stay as they were
 __device__ __forceinline__ void store_q8(uint8_t* p, u32x2 q, int n) {
   if (n >= 8) {

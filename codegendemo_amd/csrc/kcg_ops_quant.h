@@ -126,7 +126,7 @@ __device__ void swiglu_kernel(const SwigluArgs& a) {
   load8(g, in, n);
   load8(u, in + a.cols, n);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) g[i] = i < n ? g[i] / (1.f + expf(-g[i])) * u[i] : 0.f;
+  for (int i = 0; i < 8; ++i) g[i] = silu_times(g[i], u[i]);      // (behind the row: 0 times 0)
   float scale;
   const u32x2 q = quantize_group(g, scale);
   if (n > 0) {
