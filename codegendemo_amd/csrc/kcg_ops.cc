@@ -141,7 +141,6 @@ struct OnDevice {
 
 // LDS of a block of the experts' second kernel: 16 partial sums for each pair and part of I, of which there are tokens * 16
 // at most (parts = 16 / items, and items >= topk <= 16); one form keeps h beside them.
-constexpr int64_t kMoeHLds = 64 * 1024;
 int moe_partial_bytes(int64_t tokens) { return (int)(tokens * 16 * 16 * 4); }
 int64_t moe_h_bytes(int64_t pairs, int64_t inter) { return 2 * pairs * (inter + 8) * 2; }
 
@@ -161,7 +160,7 @@ int kernels_on(const HostHip* hip, int device, const DeviceKernels** out) {
       // a block of the experts' second kernel may use more than 64 KiB of LDS, part of it dynamic
       if (e == hipSuccess && i >= kMoeDown)
         e = hip->FuncSetAttribute ? hip->FuncSetAttribute((const void*)k->fn[i], hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                          moe_partial_bytes(MOE_T) + (int)kMoeHLds)
+                                                          moe_partial_bytes(MOE_T) + MOE_H_LDS)
                                   : hipErrorNotSupported;
     }
     if (e != hipSuccess) {
@@ -381,7 +380,7 @@ int kcg_moe_layer(const kcg_moe_layer_args* p, int device, uint64_t stream) {
   const int per_block = UP_WAVES / a.split;
   // the second kernel keeps h in LDS where it fits (one token, 8 experts of 1024: 12.7 us without)
   const int64_t h_bytes = moe_h_bytes(pairs, p->inter);
-  const int in_lds = h_bytes <= kMoeHLds;
+  const int in_lds = h_bytes <= MOE_H_LDS;
   return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) {
     if (int rc = launch(hip, k.fn[kMoeUp + v], (unsigned)((row_groups + per_block - 1) / per_block), (unsigned)slots, UP_WAVES * 64, 0, stream, &a)) return rc;
     return launch(hip, k.fn[kMoeDown + 2 * v + in_lds], (unsigned)(p->hidden / 16), 1, DOWN_WAVES * 64,

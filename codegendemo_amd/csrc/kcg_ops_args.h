@@ -47,6 +47,7 @@ constexpr int MOE_K = 16;        // most experts of a token
 constexpr int MOE_ITEMS = 640;   // most runs of up to 8 tokens of one expert: one per expert, and T k / 8 more
 constexpr int UP_WAVES = 8;
 constexpr int DOWN_WAVES = 16;
+constexpr int MOE_H_LDS = 64 * 1024;   // most bytes of h that the second kernel keeps in LDS
 
 struct MoeArgs {
   const void* x;               // [T, H]

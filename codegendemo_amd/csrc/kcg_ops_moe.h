@@ -391,7 +391,7 @@ struct DownLds {
   short item_expert[MOE_ITEMS], item_first[MOE_ITEMS], item_count[MOE_ITEMS];   // up to 8 pairs of one expert
   int pair[MOE_T * MOE_K];     // pairs (t k + place) by expert, then token
   int spot[MOE_T * MOE_K];     // where a pair stands in that order
-  float prob[MOE_T * MOE_K];
+  float logit[MOE_T * MOE_K], prob[MOE_T * MOE_K];
   int wave_sum[DOWN_WAVES];
   int items;
 };
@@ -405,57 +405,63 @@ __device__ void down_kernel(const MoeArgs& a, float* partial) {
   const int pairs = a.T * a.k;                       // (at most as many as threads; experts at most half of that)
   const int my_expert = tid < pairs ? a.ids[tid] : 0;
   const float my_value = tid < pairs ? a.picked[tid] : 0.f;
-  if (tid < a.E) s.tokens[tid] = 0;
-  if (tid < pairs) s.prob[tid] = my_value;
-  __syncthreads();
-  if (tid < pairs) atomicOr(&s.tokens[my_expert], 1ull << (tid / a.k));
-  __syncthreads();
-  // the chosen experts' items side by side, and how many pairs lie in front of each expert
-  const int n = tid < a.E ? __popcll(s.tokens[tid]) : 0;
-  const int mine = (n + 7) / 8;                    // items of this thread's expert
-  int upto = n << 16 | mine;                         // inclusive sums over the wave's lanes, of pairs (<= 1024) and items (<= 512)
+  // LDS: the partial sums, then (HL) h: upper parts, then lower ones, rows 8 values longer than they are (other banks).  The
+  // workspace holds the two planes side by side, pairs * I values each (I a multiple of 16): copied 16 bytes at a time.
+  constexpr int H_CHUNKS = HL ? MOE_H_LDS / 16 / (DOWN_WAVES * 64) : 1;
+  const int per_row = a.I / 8, chunks = 2 * pairs * per_row, h_row = a.I + 8;
+  u32x4 hv[H_CHUNKS];
+  if constexpr (HL) {
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(upto, d);
-    upto += lane >= d ? o : 0;
+    for (int i = 0; i < H_CHUNKS; ++i) hv[i] = ((const u32x4_a*)a.h_hi)[min(tid + i * DOWN_WAVES * 64, chunks - 1)];
   }
-  if (lane == 63) s.wave_sum[wave] = upto;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) upto += s.wave_sum[w];
-  if (n > 0) {
-    const int first = (upto >> 16) - n, at = (upto & 0xffff) - mine;
-    s.first[tid] = first;
-    for (int i = 0; i < mine; ++i) {
-      s.item_expert[at + i] = (short)tid;
-      s.item_first[at + i] = (short)(first + i * 8);
-      s.item_count[at + i] = (short)min(8, n - i * 8);
+  if (tid < pairs) s.logit[tid] = my_value;
+  if (a.T == 1) {
+    // a token alone: its places are the items (sorting them by expert would be a fifth of the call)
+    if (tid < pairs) {
+      s.item_expert[tid] = (short)my_expert;
+      s.item_first[tid] = s.pair[tid] = s.spot[tid] = tid;
+      s.item_count[tid] = 1;
+    }
+    if (tid == 0) s.items = pairs;
+  } else {
+    if (tid < a.E) s.tokens[tid] = 0;
+    __syncthreads();
+    if (tid < pairs) atomicOr(&s.tokens[my_expert], 1ull << (tid / a.k));
+    __syncthreads();
+    // the chosen experts' items side by side, and how many pairs lie in front of each expert
+    const int n = tid < a.E ? __popcll(s.tokens[tid]) : 0;
+    const int mine = (n + 7) / 8;                    // items of this thread's expert
+    int upto = n << 16 | mine;                         // inclusive sums over the wave's lanes, of pairs (<= 1024) and items (<= 512)
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(upto, d);
+      upto += lane >= d ? o : 0;
+    }
+    if (lane == 63) s.wave_sum[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += s.wave_sum[w];
+    if (n > 0) {
+      const int first = (upto >> 16) - n, at = (upto & 0xffff) - mine;
+      s.first[tid] = first;
+      for (int i = 0; i < mine; ++i) {
+        s.item_expert[at + i] = (short)tid;
+        s.item_first[at + i] = (short)(first + i * 8);
+        s.item_count[at + i] = (short)min(8, n - i * 8);
+      }
+    }
+    if (tid == DOWN_WAVES * 64 - 1) s.items = upto & 0xffff;
+    __syncthreads();
+    if (tid < pairs) {
+      const int spot = s.first[my_expert] + __popcll(s.tokens[my_expert] & ((1ull << (tid / a.k)) - 1));
+      s.pair[spot] = tid;
+      s.spot[tid] = spot;
     }
   }
-  if (tid == DOWN_WAVES * 64 - 1) s.items = upto & 0xffff;
   __syncthreads();
-  if (tid < pairs) {
-    const int spot = s.first[my_expert] + __popcll(s.tokens[my_expert] & ((1ull << (tid / a.k)) - 1));
-    s.pair[spot] = tid;
-    s.spot[tid] = spot;
-  }
-  // the weights of the pairs (place 0 holds a token's largest logit)
-  float prob = my_value;
-  if (a.renormalize && tid < pairs) {
-    const float* l = s.prob + tid / a.k * a.k;
-    const float top = l[0];
-    float sum = 0.f;
-    for (int j = 0; j < a.k; ++j) sum += l[j] == -__builtin_inff() ? 0.f : expf(l[j] - top);
-    prob = my_value == -__builtin_inff() ? 0.f : expf(my_value - top) / sum;
-  }
-  if (blockIdx.x == 0 && tid < pairs) a.probs[tid] = prob;
-  __syncthreads();
-  if (tid < pairs) s.prob[tid] = prob;               // (read behind the barrier in front of the last sum)
   const int items = s.items;
   const int KB = (a.I + GROUP - 1) / GROUP, full = a.I / GROUP;
   const int parts = max(1, min(DOWN_WAVES / items, KB));
   const int r = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
-  // LDS: the partial sums, then (HL) h: upper parts, then lower ones, rows 8 values longer than they are (other banks)
-  const int h_row = a.I + 8;
   __bf16* h_lds = (__bf16*)(partial + pairs * parts * 16);
   struct Stage {
     Raw<W> w;
@@ -526,15 +532,27 @@ __device__ void down_kernel(const MoeArgs& a, float* partial) {
     if (decltype(i_c)::value < left) load(st[decltype(i_c)::value]);
   });
   if constexpr (HL) {
-    // (16 bytes a thread; rows of I values, I a multiple of 16)
-    const int per_row = a.I / 8, chunks = 2 * pairs * per_row;
-    for (int i = tid; i < chunks; i += DOWN_WAVES * 64) {
-      const int row = i / per_row, c = i - row * per_row;
-      const __bf16* from = (row < pairs ? (const __bf16*)a.h_hi + (int64_t)row * a.I : (const __bf16*)a.h_lo + (int64_t)(row - pairs) * a.I) + c * 8;
-      *(u32x4_a*)(h_lds + row * h_row + c * 8) = *(const u32x4_a*)from;
+#pragma unroll
+    for (int i = 0; i < H_CHUNKS; ++i) {
+      const int c = tid + i * DOWN_WAVES * 64, row = c / per_row;
+      if (c < chunks) *(u32x4_a*)(h_lds + row * h_row + (c - row * per_row) * 8) = hv[i];
     }
-    __syncthreads();
   }
+  // the weights of the pairs (place 0 holds a token's largest logit), while the first loads are on their way
+  if (tid < pairs) {
+    float prob = my_value;
+    if (a.renormalize) {
+      const float* l = s.logit + tid / a.k * a.k;
+      const float top = l[0];
+      float sum = 0.f;
+#pragma unroll 4
+      for (int j = 0; j < a.k; ++j) sum += l[j] == -__builtin_inff() ? 0.f : expf(l[j] - top);
+      prob = my_value == -__builtin_inff() ? 0.f : expf(my_value - top) / sum;
+    }
+    s.prob[tid] = prob;
+    if (blockIdx.x == 0) a.probs[tid] = prob;
+  }
+  if constexpr (HL) __syncthreads();
   for (; left >= 2 * N - 1; left -= N) {
     static_for<0, N>([&](auto i_c) {
       constexpr int i = decltype(i_c)::value;
@@ -551,6 +569,7 @@ __device__ void down_kernel(const MoeArgs& a, float* partial) {
   for (int i = tid; i < a.T * 16; i += DOWN_WAVES * 64) {
     const int t = i >> 4, c = i & 15;
     float sum = 0.f;
+#pragma unroll 4
     for (int j = 0; j < a.k; ++j) {
       const float p = s.prob[t * a.k + j];
       const float* v = partial + s.spot[t * a.k + j] * parts * 16 + c;
