@@ -1,4 +1,5 @@
 // kcg_ops.cc — host side of the operators declared in include/kcg_ops.h: argument checks, the choice of a kernel, launches.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdio>
@@ -65,7 +66,7 @@ double skinny_estimate(int rt, int64_t n, int64_t groups) {
   return 2.2 + groups * (rt == 1 ? .172 : .24) * (rounds > 1 ? rounds : 1);
 }
 
-enum { kNorm = 0, kSwiglu = kNorm + 21, kSkinny = kSwiglu + 3, kTile = kSkinny + 12, kMoeUp = kTile + 3 * kTiles, kMoeDown = kMoeUp + 3, kNumKernels = kMoeDown + 6 };
+enum { kNorm = 0, kSwiglu = kNorm + 21, kSkinny = kSwiglu + 3, kTile = kSkinny + 12, kMoeUp = kTile + 3 * kTiles, kMoeFew = kMoeUp + 3, kMoeMany = kMoeFew + 3, kMoeCombine = kMoeMany + 2, kNumKernels = kMoeCombine + 2 };
 
 std::string kernel_symbol(int i) {
   static const char* const types[3] = {"bf16", "f16", "f32"};
@@ -78,8 +79,10 @@ std::string kernel_symbol(int i) {
     return std::string("kcg_mm8_skinny_") + types[(i - kSkinny) / 4] + "_" + std::to_string(v / 2 + 1) + "x" + std::to_string(v % 2 + 1);
   }
   if (i < kMoeUp) return std::string("kcg_mm8_tile_") + types[(i - kTile) / kTiles] + "_" + kTileTable[(i - kTile) % kTiles].name;
-  if (i < kMoeDown) return std::string("kcg_moe_up_") + moe[i - kMoeUp];
-  return std::string("kcg_moe_down_") + moe[(i - kMoeDown) / 2] + "_" + std::to_string((i - kMoeDown) % 2);
+  if (i < kMoeFew) return std::string("kcg_moe_up_") + moe[i - kMoeUp];
+  if (i < kMoeMany) return std::string("kcg_moe_down_few_") + moe[i - kMoeFew];
+  if (i < kMoeCombine) return i == kMoeMany ? "kcg_moe_down_many_e4m3" : "kcg_moe_down_many_bf16";
+  return i == kMoeCombine ? "kcg_moe_combine_bf16" : "kcg_moe_combine_f16";
 }
 
 // What a product of these sizes (m, n > 0) with results of type t (0: bf16, 1: f16, 2: f32) runs.
@@ -139,10 +142,37 @@ struct OnDevice {
   }
 };
 
-// LDS of a block of the experts' second kernel: 16 partial sums for each pair and part of I, of which there are tokens * 16
-// at most (parts = 16 / items, and items >= topk <= 16); one form keeps h beside them.
+// LDS of a block of the experts' second kernel for few tokens: 16 partial sums for each pair and part of I, of which there are
+// tokens * 16 at most (parts = 16 / items, and items >= topk <= 16), and h beside them.
 int moe_partial_bytes(int64_t tokens) { return (int)(tokens * 16 * 16 * 4); }
 int64_t moe_h_bytes(int64_t pairs, int64_t inter) { return 2 * pairs * (inter + 8) * 2; }
+
+int64_t groups(int64_t n) { return (n + 127) / 128; }
+
+// How a call's workspace is laid out and its second product shared out.
+struct MoePlan {
+  int64_t slots, plane, parts_at, y_at, bytes;     // bytes of one plane of h; where the number of parts and y stand
+  bool few;                                        // h fits LDS: one kernel for the second product and the sum
+  int z, max_parts;
+};
+MoePlan moe_plan(int64_t tokens, int64_t experts, int64_t topk, int64_t hidden, int64_t inter) {
+  MoePlan m = {};
+  const int64_t pairs = tokens * topk, cols = (hidden + DOWN_MANY_COLS - 1) / DOWN_MANY_COLS;
+  m.slots = pairs < experts ? pairs : experts;
+  m.plane = pairs * inter * 2;
+  // 16 columns of out a block: with fewer blocks than compute units only the smallest calls gain (3 tokens, 2 of 8 experts of
+  // 4096 x 2048 in bf16: 63.7 us, the other way 50.5; 2 tokens, 8 of 128 experts of 1024 x 4096: 46.4, the other way 53)
+  m.few = tokens <= MOE_FEW && moe_h_bytes(pairs, inter) <= (hidden >= 16 * 256 ? MOE_H_LDS : MOE_H_LDS / 2);
+  // one block on each of the 256 compute units; waves without an item of their own share I, in parts.  There are at least
+  // `items` items: k experts, and 8 pairs an item.
+  m.z = cols >= 256 ? 1 : (int)(256 / cols);
+  const int64_t items = std::max<int64_t>(std::max<int64_t>(topk, (pairs + 7) / 8), 1);
+  m.max_parts = (int)std::max<int64_t>(1, std::min<int64_t>(m.z * DOWN_MANY_WAVES / items, groups(inter)));
+  m.parts_at = 2 * m.plane + pairs * 4;
+  m.y_at = (m.parts_at + 4 + 15) / 16 * 16;
+  m.bytes = tokens == 0 ? 0 : m.few ? m.y_at : m.y_at + m.max_parts * pairs * hidden * 4;
+  return m;
+}
 
 // The kernels on `device` (current): loaded once per process and device, kept until the process ends.
 int kernels_on(const HostHip* hip, int device, const DeviceKernels** out) {
@@ -157,10 +187,10 @@ int kernels_on(const HostHip* hip, int device, const DeviceKernels** out) {
     for (int i = 0; i < kNumKernels && e == hipSuccess; ++i) {
       if (i >= kTile + 2 * kTiles + kTilesF32 && i < kMoeUp) continue;       // tiles without a form for float32 results
       e = hip->ModuleGetFunction(&k->fn[i], k->module, kernel_symbol(i).c_str());
-      // a block of the experts' second kernel may use more than 64 KiB of LDS, part of it dynamic
-      if (e == hipSuccess && i >= kMoeDown)
+      // a block of the experts' second kernel for few tokens may use more than 64 KiB of LDS, part of it dynamic
+      if (e == hipSuccess && i >= kMoeFew && i < kMoeMany)
         e = hip->FuncSetAttribute ? hip->FuncSetAttribute((const void*)k->fn[i], hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                          moe_partial_bytes(MOE_T) + MOE_H_LDS)
+                                                          moe_partial_bytes(MOE_FEW) + MOE_H_LDS)
                                   : hipErrorNotSupported;
     }
     if (e != hipSuccess) {
@@ -215,7 +245,6 @@ bool extent_ok(int64_t n) { return n >= 0 && n <= kMaxExtent; }
 bool stride_ok(int64_t stride, int64_t cols, int64_t rows) { return stride >= 0 && stride <= kMaxStride && (rows <= 1 || stride >= cols); }
 bool any_stride_ok(int64_t s) { return s >= 0 && s <= kMaxStride; }
 bool aligned(int64_t p, int64_t to) { return p % to == 0; }
-int64_t groups(int64_t n) { return (n + 127) / 128; }
 
 // output scales [rows, groups]: no two of them in one place
 bool scale_layout_ok(int64_t row, int64_t group, int64_t rows, int64_t ng) {
@@ -336,8 +365,7 @@ int64_t kcg_moe_workspace_bytes(int64_t tokens, int64_t experts, int64_t topk, i
   if (topk < 1 || topk > MOE_K || topk > experts) return bad("moe_layer: topk must be in [1, 16] and at most experts");
   if (hidden < 16 || hidden % 16 || hidden > (1 << 20) || inter < 16 || inter % 16 || inter > (1 << 20))
     return bad("moe_layer: hidden and inter must be multiples of 16, at most 2^20");
-  const int64_t bytes = 2 * (tokens * topk * inter * 2) + tokens * topk * 4;
-  return (bytes + 15) / 16 * 16;
+  return moe_plan(tokens, experts, topk, hidden, inter).bytes;
 }
 
 int kcg_moe_layer(const kcg_moe_layer_args* p, int device, uint64_t stream) {
@@ -364,27 +392,27 @@ int kcg_moe_layer(const kcg_moe_layer_args* p, int device, uint64_t stream) {
       !any_stride_ok(p->w13_stride_expert) || !any_stride_ok(p->w13_stride_row) || !any_stride_ok(p->w2_stride_expert) ||
       !any_stride_ok(p->w2_stride_row))
     return bad("moe_layer: a stride is negative, or rows of out overlap");
-  const int64_t pairs = p->tokens * p->topk, slots = pairs < p->experts ? pairs : p->experts;
+  const MoePlan m = moe_plan(p->tokens, p->experts, p->topk, p->hidden, p->inter);
   char* ws = (char*)p->workspace;
-  const int64_t plane = pairs * p->inter * 2;
   MoeArgs a = {(const void*)p->x, (const float*)p->logits, (const void*)p->w13, (const void*)p->w2, (const float*)p->w13_scale, (const float*)p->w2_scale,
-               (void*)p->out, (int32_t*)p->ids, (float*)p->probs, ws, ws + plane, (float*)(ws + 2 * plane), p->x_stride, p->logits_stride, p->out_stride, p->w13_stride_expert,
-               p->w13_stride_row, p->w2_stride_expert, p->w2_stride_row, (int)p->tokens, (int)p->experts, (int)p->topk, (int)p->hidden,
-               (int)p->inter, (int)slots, p->renormalize != 0, UP_WAVES, 1};
+               (void*)p->out, (int32_t*)p->ids, (float*)p->probs, ws, ws + m.plane, (float*)(ws + 2 * m.plane), (int*)(ws + m.parts_at), (float*)(ws + m.y_at),
+               p->x_stride, p->logits_stride, p->out_stride, p->w13_stride_expert, p->w13_stride_row, p->w2_stride_expert, p->w2_stride_row,
+               (int)p->tokens, (int)p->experts, (int)p->topk, (int)p->hidden, (int)p->inter, (int)m.slots, p->renormalize != 0, 2, m.max_parts};
   // Waves that share 16 rows of the first product: as few as leave 4096 waves to the chip, two at least (at 64 tokens, 128
   // experts of 1024 x 4096: 220 us with one, 196 with two, 215 with four, 260 with eight; at one token, 8 of 64 experts
   // of 1024 x 2048: 23.2, 14.8, 10.4 and 9.9).
   const int64_t row_groups = p->inter / 16;
-  a.split = 2;
-  while (a.split < UP_WAVES && row_groups * slots * a.split < 4096) a.split *= 2;
+  while (a.split < UP_WAVES && row_groups * m.slots * a.split < 4096) a.split *= 2;
   const int per_block = UP_WAVES / a.split;
-  // the second kernel keeps h in LDS where it fits (one token, 8 experts of 1024: 12.7 us without)
-  const int64_t h_bytes = moe_h_bytes(pairs, p->inter);
-  const int in_lds = h_bytes <= MOE_H_LDS;
   return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) {
-    if (int rc = launch(hip, k.fn[kMoeUp + v], (unsigned)((row_groups + per_block - 1) / per_block), (unsigned)slots, UP_WAVES * 64, 0, stream, &a)) return rc;
-    return launch(hip, k.fn[kMoeDown + 2 * v + in_lds], (unsigned)(p->hidden / 16), 1, DOWN_WAVES * 64,
-                  moe_partial_bytes(p->tokens) + (in_lds ? (int)h_bytes : 0), stream, &a);
+    if (int rc = launch(hip, k.fn[kMoeUp + v], (unsigned)((row_groups + per_block - 1) / per_block), (unsigned)m.slots, UP_WAVES * 64, 0, stream, &a)) return rc;
+    if (m.few)
+      return launch(hip, k.fn[kMoeFew + v], (unsigned)(p->hidden / 16), 1, DOWN_WAVES * 64,
+                    moe_partial_bytes(p->tokens) + (int)moe_h_bytes(p->tokens * p->topk, p->inter), stream, &a);
+    if (int rc = launch(hip, k.fn[kMoeMany + (v == 2)], (unsigned)((p->hidden + DOWN_MANY_COLS - 1) / DOWN_MANY_COLS), (unsigned)m.z, DOWN_MANY_WAVES * 64, 0,
+                        stream, &a))
+      return rc;
+    return launch(hip, k.fn[kMoeCombine + (v == 1)], (unsigned)((p->hidden + 1023) / 1024), (unsigned)p->tokens, 256, 0, stream, &a);
   });
 }
 

@@ -46,14 +46,15 @@ TILE(_Float16, f16, 128, 128, 4, 2, 4, 1, 2) TILE(_Float16, f16, 256, 256, 4, 2,
 
 #define MOE(OPS, W, X, NAME)                                                                                        \
   extern "C" __global__ void __launch_bounds__(UP_WAVES * 64, 4) kcg_moe_up_##NAME(MoeArgs a) { up_kernel<OPS, W, X>(a); } \
-  extern "C" __global__ void __launch_bounds__(DOWN_WAVES * 64) kcg_moe_down_##NAME##_0(MoeArgs a) {                \
+  extern "C" __global__ void __launch_bounds__(DOWN_WAVES * 64) kcg_moe_down_few_##NAME(MoeArgs a) {               \
     extern __shared__ __attribute__((aligned(16))) float partial[];                                                 \
-    down_kernel<W, X, false>(a, partial);                                                                           \
-  }                                                                                                                 \
-  extern "C" __global__ void __launch_bounds__(DOWN_WAVES * 64) kcg_moe_down_##NAME##_1(MoeArgs a) {                \
-    extern __shared__ __attribute__((aligned(16))) float partial[];                                                 \
-    down_kernel<W, X, true>(a, partial);                                                                            \
+    down_few_kernel<W, X>(a, partial);                                                                              \
   }
 MOE(Bf16Ops, uint8_t, __bf16, e4m3_bf16)
 MOE(F16Ops, uint8_t, _Float16, e4m3_f16)
 MOE(Bf16Ops, __bf16, __bf16, bf16_bf16)
+// (these keep nothing in x's type)
+extern "C" __global__ void __launch_bounds__(DOWN_MANY_WAVES * 64, 2) kcg_moe_down_many_e4m3(MoeArgs a) { down_many_kernel<uint8_t>(a); }
+extern "C" __global__ void __launch_bounds__(DOWN_MANY_WAVES * 64, 2) kcg_moe_down_many_bf16(MoeArgs a) { down_many_kernel<__bf16>(a); }
+extern "C" __global__ void __launch_bounds__(256) kcg_moe_combine_bf16(MoeArgs a) { combine_kernel<__bf16>(a); }
+extern "C" __global__ void __launch_bounds__(256) kcg_moe_combine_f16(MoeArgs a) { combine_kernel<_Float16>(a); }

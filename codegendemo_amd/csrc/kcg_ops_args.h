@@ -47,7 +47,10 @@ constexpr int MOE_K = 16;        // most experts of a token
 constexpr int MOE_ITEMS = 640;   // most runs of up to 8 tokens of one expert: one per expert, and T k / 8 more
 constexpr int UP_WAVES = 8;
 constexpr int DOWN_WAVES = 16;
-constexpr int MOE_H_LDS = 64 * 1024;   // most bytes of h that the second kernel keeps in LDS
+constexpr int MOE_FEW = 4;             // most tokens of the second kernel for few tokens, and most bytes of h that it keeps in LDS
+constexpr int MOE_H_LDS = 128 * 1024;
+constexpr int DOWN_MANY_WAVES = 8;
+constexpr int DOWN_MANY_COLS = 64;     // columns of out a block of the second kernel for more tokens makes
 
 struct MoeArgs {
   const void* x;               // [T, H]
@@ -62,11 +65,14 @@ struct MoeArgs {
   void* h_hi;                  // workspace: [T k, I] twice
   void* h_lo;
   float* picked;               // workspace: [T, k] logits of the chosen (renormalised) or their probabilities
+  int* parts;                  // workspace: how many parts of I there are
+  float* y;                    // workspace: [parts, T, k, H] products, to be weighed and added
   int64_t x_stride, logits_stride, out_stride;
   int64_t w13_e, w13_r, w2_e, w2_r;     // elements from expert to expert, row to row
   int T, E, k, H, I, slots;
   int renormalize;
-  int split, rounds;           // first kernel: waves that share 16 rows, sets of rows a block takes one after another
+  int split;                   // first kernel: waves that share 16 rows (>= 2)
+  int max_parts;               // second kernel for more tokens: most parts of I that y has room for
 };
 
 }  // namespace kcg_ops

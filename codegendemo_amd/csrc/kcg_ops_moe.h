@@ -1,6 +1,6 @@
-// kcg_ops_moe.h — a layer of routed experts for a few tokens (T <= 64), in two kernels:
+// kcg_ops_moe.h — a layer of routed experts for a few tokens (T <= 64), in two kernels, or three:
 //   up:   h[t, j] = silu(W1_e x_t) * (W3_e x_t)           for the j-th expert e of token t
-//   down: out[t]  = sum_j p[t, j] W2_e h[t, j]
+//   down: out[t]  = sum_j p[t, j] W2_e h[t, j]            one kernel for a few tokens, else products and their sum apart
 // Bound by the bytes of the experts that at least one token chose: every such weight is read once, by one block, straight
 // into the matrix operand.  8-bit weights become bf16 (fp16 where x is fp16) on the way, which holds e4m3 exactly; their
 // block scale multiplies the fp32 sum of the 128 products that share it.  h is kept as two bf16 numbers, its rounding and
@@ -196,17 +196,14 @@ __device__ __forceinline__ int route(const MoeArgs& a, RouteLds& s, int slot, bo
 
 // ---- up ------------------------------------------------------------------------------------------
 // grid (x, slots), UP_WAVES waves.  A row group is 16 gate rows and the 16 up rows beside them.  `split` waves share a row
-// group, each with a part of H, and meet in LDS; UP_WAVES / split row groups run side by side, and a block takes `rounds` such
-// sets one after another.  split = 1 needs no barrier and lets every wave stream on its own: for calls with rows enough; a
-// single token's few rows take split = UP_WAVES.  The loads of a step (a group of 128 of one row group) are issued before the
-// products of the step in front of it, across row groups too (up to 16 tokens).
+// group, each with a part of H, and meet in LDS; UP_WAVES / split row groups run side by side.  The loads of a step (a group of
+// 128 of one row group) are issued before the products of the step in front of it (up to 16 tokens).
 template <class Ops, class W, class X, int CT>
 __device__ __forceinline__ void up_tiles(const MoeArgs& a, RouteLds& s, f32x4* red, int ex, int count, int skip) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, g = lane >> 4;
   const int split = a.split, side = UP_WAVES / split;
-  const int rg_end = a.I / 16, rounds = a.rounds;
-  const int rg0 = blockIdx.x * side * rounds + wave / split, part = wave % split;
+  const int rg_end = a.I / 16, rg = blockIdx.x * side + wave / split, part = wave % split;
   const W* wg = (const W*)a.w13 + ex * a.w13_e + (int64_t)r * a.w13_r;
   const int KB = (a.H + GROUP - 1) / GROUP, full = a.H / GROUP;
   const float* sc = sizeof(W) == 1 ? a.s13 + (int64_t)ex * ((2 * a.I + GROUP - 1) / GROUP) * KB : nullptr;
@@ -218,17 +215,19 @@ __device__ __forceinline__ void up_tiles(const MoeArgs& a, RouteLds& s, f32x4* r
     RawValues x[CT];
     float vg, vu;
   };
-  auto load = [&](Stage& st, int rg, int kb) {
-    const W* rowg = wg + (int64_t)rg * 16 * a.w13_r;
-    const W* rowu = rowg + (int64_t)a.I * a.w13_r;
+  // (a row group behind the last one is computed from the last one's weights and not stored: there are barriers below)
+  const int rgl = min(rg, rg_end - 1);
+  const W* rowg = wg + (int64_t)rgl * 16 * a.w13_r;
+  const W* rowu = rowg + (int64_t)a.I * a.w13_r;
+  auto load = [&](Stage& st, int kb) {
     st.g = load_w<W>(rowg, kb * GROUP, g, a.H);
     st.u = load_w<W>(rowu, kb * GROUP, g, a.H);
 #pragma unroll
     for (int c = 0; c < CT; ++c) st.x[c] = load_x<W>(x[c], kb * GROUP, g, a.H);
     if constexpr (sizeof(W) == 1) {
       // (16 rows from a multiple of 16 lie in one block of 128)
-      st.vg = sc[(int64_t)(rg * 16 / GROUP) * KB + kb];
-      st.vu = sc[(int64_t)((a.I + rg * 16) / GROUP) * KB + kb];
+      st.vg = sc[(int64_t)(rgl * 16 / GROUP) * KB + kb];
+      st.vu = sc[(int64_t)((a.I + rgl * 16) / GROUP) * KB + kb];
     }
   };
   auto write = [&](int n, int row, float gate, float up) {
@@ -241,10 +240,8 @@ __device__ __forceinline__ void up_tiles(const MoeArgs& a, RouteLds& s, f32x4* r
     ((__bf16*)a.h_lo)[o] = __builtin_isfinite(hf) ? (__bf16)(h - hf) : (__bf16)0.f;
   };
   f32x4 ag[CT], au[CT];
-  auto start = [&]() {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) ag[c] = au[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  };
+  for (int c = 0; c < CT; ++c) ag[c] = au[c] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](Stage& st, int kb) {
     if (kb >= full) {
       clear_tail<W>(st.g, kb * GROUP, g, a.H);
@@ -277,91 +274,50 @@ __device__ __forceinline__ void up_tiles(const MoeArgs& a, RouteLds& s, f32x4* r
       }
     }
   };
-  // the sums of a row group become h
-  auto finish = [&](int round, int rg) {
-    if (split == 1) {
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const int n = skip + c * 16 + r;
-        if (n < count) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) write(n, rg * 16 + g * 4 + i, ag[c][i], au[c][i]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        __syncthreads();                              // (the sums of the tile before have been read)
-        red[wave * 128 + lane] = ag[c];
-        red[wave * 128 + 64 + lane] = au[c];
-        __syncthreads();
-        // thread -> row % 16 of column / 16 of a row group; element (row % 4) of the lane that holds it
-        for (int i = tid; i < side * 256; i += UP_WAVES * 64) {
-          const int q = i >> 8, row = i & 15, col = (i >> 4) & 15, at = (row >> 2) * 16 + col;
-          float gate = 0.f, up = 0.f;
-          for (int w = q * split; w < (q + 1) * split; ++w) {
-            gate += red[w * 128 + at][row & 3];
-            up += red[w * 128 + 64 + at][row & 3];
-          }
-          const int n = skip + c * 16 + col, to_rg = blockIdx.x * side * rounds + round * side + q;
-          if (n < count && to_rg < rg_end) write(n, to_rg * 16 + row, gate, up);
-        }
-      }
-    }
-  };
-  const int from = KB * part / split, to = KB * (part + 1) / split;
-  // Every wave runs the same number of rounds, row groups behind the last one among them (there are barriers inside; such a
-  // row group is computed from the last one's weights and not stored).
-  int round = 0, kb = from;                            // of the next products
-  auto step = [&](Stage& st) {
-    if (kb == from) start();
-    multiply(st, kb);
-    if (++kb == to) {
-      const int rg = rg0 + round * side;
-      if (split > 1 || rg < rg_end) finish(round, rg);
-      ++round;
-      kb = from;
-    }
-  };
-  int load_round = 0, load_kb = from;
-  auto fetch = [&](Stage& st) {
-    load(st, min(rg0 + load_round * side, rg_end - 1), load_kb);
-    if (++load_kb == to) {
-      ++load_round;
-      load_kb = from;
-    }
-  };
-  int left = rounds * (to - from);
-  if (left == 0) {
-    for (; round < rounds; ++round) {
-      start();
-      if (split > 1) finish(round, rg0 + round * side);
-    }
-    return;
-  }
+  int kb = KB * part / split;
+  const int to = KB * (part + 1) / split;
   if constexpr (CT == 1) {
     // (two named stages in turn: copying one into the other would wait for its loads)
     Stage a0, a1;
-    fetch(a0);
-    for (; left > 2; left -= 2) {
-      fetch(a1);
-      step(a0);
-      fetch(a0);
-      step(a1);
+    if (kb < to) load(a0, kb);
+    for (; kb + 2 < to; kb += 2) {
+      load(a1, kb + 1);
+      multiply(a0, kb);
+      load(a0, kb + 2);
+      multiply(a1, kb + 1);
     }
-    if (left == 2) {
-      fetch(a1);
-      step(a0);
-      step(a1);
-    } else {
-      step(a0);
+    if (kb + 2 == to) {
+      load(a1, kb + 1);
+      multiply(a0, kb);
+      multiply(a1, kb + 1);
+    } else if (kb < to) {
+      multiply(a0, kb);
     }
   } else {
     // (two stages of two column tiles would not fit the registers of 16 waves a compute unit)
-    for (; left > 0; --left) {
+    for (; kb < to; ++kb) {
       Stage now;
-      fetch(now);
-      step(now);
+      load(now, kb);
+      multiply(now, kb);
+    }
+  }
+  // the sums become h
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    __syncthreads();                              // (the sums of the tile before have been read)
+    red[wave * 128 + lane] = ag[c];
+    red[wave * 128 + 64 + lane] = au[c];
+    __syncthreads();
+    // thread -> row % 16 of column / 16 of a row group; element (row % 4) of the lane that holds it
+    for (int i = tid; i < side * 256; i += UP_WAVES * 64) {
+      const int q = i >> 8, row = i & 15, col = (i >> 4) & 15, at = (row >> 2) * 16 + col;
+      float gate = 0.f, up = 0.f;
+      for (int w = q * split; w < (q + 1) * split; ++w) {
+        gate += red[w * 128 + at][row & 3];
+        up += red[w * 128 + 64 + at][row & 3];
+      }
+      const int n = skip + c * 16 + col, to_rg = blockIdx.x * side + q;
+      if (n < count && to_rg < rg_end) write(n, to_rg * 16 + row, gate, up);
     }
   }
 }
@@ -381,204 +337,310 @@ __device__ void up_kernel(const MoeArgs& a) {
 }
 
 // ---- down ----------------------------------------------------------------------------------------
-// grid H / 16: a block makes 16 columns of every token's row.  Work items are (expert, up to 8 of its tokens, part of I): the
-// 16 columns of a product hold the upper parts of 8 tokens' h and beside them the lower ones, whose sums are added at the
-// end, so that a group of 128 costs four loads of h and not eight (the loads, not the bytes, are what limits here: eight took
-// 167 us where four of them left out took 129, at 128 experts of 4096 x 1024).  The waves take the items in turn, put their partial sums side by side in LDS, and the sum over parts and places runs in a fixed order.
-struct DownLds {
+// Work items are (expert, up to 8 of its tokens): the 16 columns of a product hold the upper parts of 8 tokens' h and beside
+// them the lower ones, whose sums are added at the end, so that a group of 128 costs four loads of h and not eight.  Waves
+// take (item, part of I) in turn; sums over parts and over a token's places run in a fixed order.
+struct SortLds {
   unsigned long long tokens[MOE_E];   // which tokens chose the expert
   int first[MOE_E];            // pairs of the experts in front of it
   short item_expert[MOE_ITEMS], item_first[MOE_ITEMS], item_count[MOE_ITEMS];   // up to 8 pairs of one expert
   int pair[MOE_T * MOE_K];     // pairs (t k + place) by expert, then token
-  int spot[MOE_T * MOE_K];     // where a pair stands in that order
-  float logit[MOE_T * MOE_K], prob[MOE_T * MOE_K];
   int wave_sum[DOWN_WAVES];
   int items;
 };
 
-// HL: h of the whole call fits LDS (a token or two): the block copies it there once and the waves' loads are the weights
-// alone, four steps of them in flight; else h comes from memory beside the weights, two steps in flight.
-template <class W, class X, bool HL>
-__device__ void down_kernel(const MoeArgs& a, float* partial) {
-  __shared__ DownLds s;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int pairs = a.T * a.k;                       // (at most as many as threads; experts at most half of that)
-  const int my_expert = tid < pairs ? a.ids[tid] : 0;
-  const float my_value = tid < pairs ? a.picked[tid] : 0.f;
-  // LDS: the partial sums, then (HL) h: upper parts, then lower ones, rows 8 values longer than they are (other banks).  The
-  // workspace holds the two planes side by side, pairs * I values each (I a multiple of 16): copied 16 bytes at a time.
-  constexpr int H_CHUNKS = HL ? MOE_H_LDS / 16 / (DOWN_WAVES * 64) : 1;
-  const int per_row = a.I / 8, chunks = 2 * pairs * per_row, h_row = a.I + 8;
-  u32x4 hv[H_CHUNKS];
-  if constexpr (HL) {
-#pragma unroll
-    for (int i = 0; i < H_CHUNKS; ++i) hv[i] = ((const u32x4_a*)a.h_hi)[min(tid + i * DOWN_WAVES * 64, chunks - 1)];
-  }
-  if (tid < pairs) s.logit[tid] = my_value;
+// The pairs in the order of their experts, cut into items; NT >= MOE_E threads, thread i has the experts of pairs i, i + NT, ...
+// Ends with a barrier; at(pair, spot) is told where each pair stands.
+template <int NT, class F>
+__device__ __forceinline__ void sort_pairs(const MoeArgs& a, SortLds& s, const int (&expert)[MOE_T * MOE_K / NT], F&& at_spot) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pairs = a.T * a.k;
   if (a.T == 1) {
     // a token alone: its places are the items (sorting them by expert would be a fifth of the call)
     if (tid < pairs) {
-      s.item_expert[tid] = (short)my_expert;
-      s.item_first[tid] = s.pair[tid] = s.spot[tid] = tid;
+      s.item_expert[tid] = (short)expert[0];
+      s.item_first[tid] = s.pair[tid] = tid;
       s.item_count[tid] = 1;
+      at_spot(tid, tid);
     }
     if (tid == 0) s.items = pairs;
-  } else {
-    if (tid < a.E) s.tokens[tid] = 0;
     __syncthreads();
-    if (tid < pairs) atomicOr(&s.tokens[my_expert], 1ull << (tid / a.k));
-    __syncthreads();
-    // the chosen experts' items side by side, and how many pairs lie in front of each expert
-    const int n = tid < a.E ? __popcll(s.tokens[tid]) : 0;
-    const int mine = (n + 7) / 8;                    // items of this thread's expert
-    int upto = n << 16 | mine;                         // inclusive sums over the wave's lanes, of pairs (<= 1024) and items (<= 512)
+    return;
+  }
+  if (tid < a.E) s.tokens[tid] = 0;
+  __syncthreads();
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(upto, d);
-      upto += lane >= d ? o : 0;
+  for (int i = 0; i < MOE_T * MOE_K / NT; ++i)
+    if (tid + i * NT < pairs) atomicOr(&s.tokens[expert[i]], 1ull << ((tid + i * NT) / a.k));
+  __syncthreads();
+  // the chosen experts' items side by side, and how many pairs lie in front of each expert
+  const int n = tid < a.E ? __popcll(s.tokens[tid]) : 0;
+  const int mine = (n + 7) / 8;                    // items of this thread's expert
+  int upto = n << 16 | mine;                       // inclusive sums over the wave's lanes, of pairs (<= 1024) and items (<= 512)
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(upto, d);
+    upto += lane >= d ? o : 0;
+  }
+  if (lane == 63) s.wave_sum[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) upto += s.wave_sum[w];
+  if (n > 0) {
+    const int first = (upto >> 16) - n, at = (upto & 0xffff) - mine;
+    s.first[tid] = first;
+    for (int i = 0; i < mine; ++i) {
+      s.item_expert[at + i] = (short)tid;
+      s.item_first[at + i] = (short)(first + i * 8);
+      s.item_count[at + i] = (short)min(8, n - i * 8);
     }
-    if (lane == 63) s.wave_sum[wave] = upto;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) upto += s.wave_sum[w];
-    if (n > 0) {
-      const int first = (upto >> 16) - n, at = (upto & 0xffff) - mine;
-      s.first[tid] = first;
-      for (int i = 0; i < mine; ++i) {
-        s.item_expert[at + i] = (short)tid;
-        s.item_first[at + i] = (short)(first + i * 8);
-        s.item_count[at + i] = (short)min(8, n - i * 8);
-      }
-    }
-    if (tid == DOWN_WAVES * 64 - 1) s.items = upto & 0xffff;
-    __syncthreads();
-    if (tid < pairs) {
-      const int spot = s.first[my_expert] + __popcll(s.tokens[my_expert] & ((1ull << (tid / a.k)) - 1));
-      s.pair[spot] = tid;
-      s.spot[tid] = spot;
+  }
+  if (tid == NT - 1) s.items = upto & 0xffff;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < MOE_T * MOE_K / NT; ++i) {
+    const int pair = tid + i * NT;
+    if (pair < pairs) {
+      const int spot = s.first[expert[i]] + __popcll(s.tokens[expert[i]] & ((1ull << (pair / a.k)) - 1));
+      s.pair[spot] = pair;
+      at_spot(pair, spot);
     }
   }
   __syncthreads();
-  const int items = s.items;
-  const int KB = (a.I + GROUP - 1) / GROUP, full = a.I / GROUP;
-  const int parts = max(1, min(DOWN_WAVES / items, KB));
-  const int r = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
-  __bf16* h_lds = (__bf16*)(partial + pairs * parts * 16);
+}
+
+// the weight of place `place` of a token, from what the first kernel picked for its k places (place 0 holds the largest logit)
+__device__ __forceinline__ float pair_weight(const MoeArgs& a, const float* picked, int place) {
+  const float mine = picked[place];
+  if (!a.renormalize) return mine;
+  const float top = picked[0];
+  float sum = 0.f;
+#pragma unroll 4
+  for (int j = 0; j < a.k; ++j) sum += picked[j] == -__builtin_inff() ? 0.f : expf(picked[j] - top);
+  return mine == -__builtin_inff() ? 0.f : expf(mine - top) / sum;
+}
+
+// One (item, part of I) after another of a wave's share, RT tiles of 16 rows of W2 from row `n0` on beside each other.  The loads
+// of a step are issued N - 1 steps before its products, across items too (named stages in turn: copying one into another
+// would wait for its loads).  HL: h lies in LDS, and the loads are the weights alone.
+template <class W, int RT, int N, bool HL>
+struct DownWave {
   struct Stage {
-    Raw<W> w;
+    Raw<W> w[RT];
     RawValues h;                                     // (HL: read when it is used)
     const __bf16* row;
     float v;
-    int kb, item;                                    // item: -1 - item in its last step
+    int kb, unit;                                    // unit: -1 - unit in its last step
   };
+  const MoeArgs& a;
+  const SortLds& s;
+  const __bf16* h_lds;
+  const int lane, r, g, KB, full, parts, units, stride, n0;
+  int64_t w_row[RT];
+  Stage st[N];
+  f32x4 acc[RT];
   // where the loads of the wave's next step come from
   const W* w = nullptr;
   const float* sc = nullptr;
   const __bf16* h = nullptr;
-  int item = wave, kb = 0, to = 0;
-  auto open = [&]() {
-    if (item >= items * parts) return;
-    const int which = item / parts, part = item - which * parts;
+  int unit, kb = 0, to = 0, left = 0;
+
+  __device__ __forceinline__ DownWave(const MoeArgs& args, const SortLds& sort, const __bf16* hl, int row0, int part_count, int first, int step)
+      : a(args), s(sort), h_lds(hl), lane(threadIdx.x & 63), r(lane & 15), g(lane >> 4), KB((a.I + GROUP - 1) / GROUP), full(a.I / GROUP),
+        parts(part_count), units(sort.items * part_count), stride(step), n0(row0), unit(first) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      w_row[t] = (int64_t)min(n0 + t * 16 + r, a.H - 1) * a.w2_r;       // (rows behind the last one are not stored)
+      acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int u = first; u < units; u += step) {
+      const int part = u % parts;
+      left += KB * (part + 1) / parts - KB * part / parts;
+    }
+    open();
+    static_for<0, N - 1>([&](auto i_c) {
+      if (decltype(i_c)::value < left) load(st[decltype(i_c)::value]);
+    });
+  }
+  __device__ __forceinline__ void open() {
+    if (unit >= units) return;
+    const int which = unit / parts, part = unit - which * parts;
     const int ex = __builtin_amdgcn_readfirstlane(s.item_expert[which]), first = __builtin_amdgcn_readfirstlane(s.item_first[which]);
     const int count = __builtin_amdgcn_readfirstlane(s.item_count[which]);
-    w = (const W*)a.w2 + ex * a.w2_e + (int64_t)(n0 + r) * a.w2_r;
+    w = (const W*)a.w2 + ex * a.w2_e;
+    // (RT tiles of 16 rows from a multiple of RT tiles lie in one block of 128)
     if constexpr (sizeof(W) == 1) sc = a.s2 + ((int64_t)ex * ((a.H + GROUP - 1) / GROUP) + n0 / GROUP) * KB;
     const int pair = s.pair[first + min(r & 7, count - 1)];
-    if constexpr (HL) h = h_lds + (pair + (r < 8 ? 0 : pairs)) * h_row;
+    if constexpr (HL) h = h_lds + (pair + (r < 8 ? 0 : a.T * a.k)) * (a.I + 8);
     else h = (const __bf16*)(r < 8 ? a.h_hi : a.h_lo) + (int64_t)pair * a.I;
     kb = KB * part / parts;
     to = KB * (part + 1) / parts;
-  };
-  auto load = [&](Stage& st) {
-    st.w = load_w<W>(w, kb * GROUP, g, a.I);
-    if constexpr (HL) st.row = h;
-    else st.h = load_x<W>(h, kb * GROUP, g, a.I);
-    if constexpr (sizeof(W) == 1) st.v = sc[kb];
-    st.kb = kb;
-    st.item = item;
+  }
+  __device__ __forceinline__ void load(Stage& q) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) q.w[t] = load_w<W>(w + w_row[t], kb * GROUP, g, a.I);
+    if constexpr (HL) q.row = h;
+    else q.h = load_x<W>(h, kb * GROUP, g, a.I);
+    if constexpr (sizeof(W) == 1) q.v = sc[kb];
+    q.kb = kb;
+    q.unit = unit;
     if (++kb == to) {
-      st.item = -1 - item;
-      item += DOWN_WAVES;
+      q.unit = -1 - unit;
+      unit += stride;
       open();
     }
-  };
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](Stage& st) {
-    if (st.kb >= full) clear_tail<W>(st.w, st.kb * GROUP, g, a.I);
-    if constexpr (HL) st.h = load_x<W>(st.row, st.kb * GROUP, g, a.I);
-    f32x4 d = sizeof(W) == 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) d = Bf16Ops::mma(operand<Bf16Ops, W>(st.w, i), __builtin_bit_cast(bf16x8, st.h.v[i]), d);
-    if constexpr (sizeof(W) == 1) add_scaled(acc, d, st.v);
-    else acc = d;
-    if (st.item < 0) {
-      const int done = -1 - st.item, which = done / parts, part = done - which * parts;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(acc[i]), 0x128, 0xf, 0xf, false));   // row_ror:8
-      if (r < s.item_count[which]) *(f32x4*)(partial + (((s.item_first[which] + r) * parts + part) * 16 + g * 4)) = acc;
-      acc = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-  };
-  // The loads of a step are issued N - 1 steps before its products, across items too (named stages in turn: copying one into
-  // another would wait for its loads).
-  int left = 0;
-  for (int i = wave; i < items * parts; i += DOWN_WAVES) {
-    const int part = i % parts;
-    left += KB * (part + 1) / parts - KB * part / parts;
   }
-  constexpr int N = HL ? 4 : 2;
-  Stage st[N];
-  open();
-  static_for<0, N - 1>([&](auto i_c) {
-    if (decltype(i_c)::value < left) load(st[decltype(i_c)::value]);
-  });
-  if constexpr (HL) {
+  // done(unit's item, part, sums of tile t: lane (r, g) has rows 4 g .. 4 g + 3 of the item's pair r, r < 8)
+  template <class F>
+  __device__ __forceinline__ void multiply(Stage& q, F&& done) {
+    if (q.kb >= full)
 #pragma unroll
-    for (int i = 0; i < H_CHUNKS; ++i) {
-      const int c = tid + i * DOWN_WAVES * 64, row = c / per_row;
-      if (c < chunks) *(u32x4_a*)(h_lds + row * h_row + (c - row * per_row) * 8) = hv[i];
+      for (int t = 0; t < RT; ++t) clear_tail<W>(q.w[t], q.kb * GROUP, g, a.I);
+    if constexpr (HL) q.h = load_x<W>(q.row, q.kb * GROUP, g, a.I);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      f32x4 d = sizeof(W) == 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[t];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d = Bf16Ops::mma(operand<Bf16Ops, W>(q.w[t], i), __builtin_bit_cast(bf16x8, q.h.v[i]), d);
+      if constexpr (sizeof(W) == 1) add_scaled(acc[t], d, q.v);
+      else acc[t] = d;
+    }
+    if (q.unit < 0) {
+      const int unit = -1 - q.unit, which = unit / parts;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(acc[t][i]), 0x128, 0xf, 0xf, false));   // row_ror:8
+        done(which, unit - which * parts, t, acc[t]);
+        acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
     }
   }
-  // the weights of the pairs (place 0 holds a token's largest logit), while the first loads are on their way
-  if (tid < pairs) {
-    float prob = my_value;
-    if (a.renormalize) {
-      const float* l = s.logit + tid / a.k * a.k;
-      const float top = l[0];
-      float sum = 0.f;
-#pragma unroll 4
-      for (int j = 0; j < a.k; ++j) sum += l[j] == -__builtin_inff() ? 0.f : expf(l[j] - top);
-      prob = my_value == -__builtin_inff() ? 0.f : expf(my_value - top) / sum;
+  template <class F>
+  __device__ __forceinline__ void run(F&& done) {
+    for (; left >= 2 * N - 1; left -= N) {
+      static_for<0, N>([&](auto i_c) {
+        constexpr int i = decltype(i_c)::value;
+        load(st[(i + N - 1) % N]);
+        multiply(st[i], done);
+      });
     }
-    s.prob[tid] = prob;
-    if (blockIdx.x == 0) a.probs[tid] = prob;
-  }
-  if constexpr (HL) __syncthreads();
-  for (; left >= 2 * N - 1; left -= N) {
-    static_for<0, N>([&](auto i_c) {
+    static_for<0, 2 * N - 2>([&](auto i_c) {
       constexpr int i = decltype(i_c)::value;
-      load(st[(i + N - 1) % N]);
-      multiply(st[i]);
+      if (i + N - 1 < left) load(st[(i + N - 1) % N]);
+      if (i < left) multiply(st[i % N], done);
     });
   }
-  static_for<0, 2 * N - 2>([&](auto i_c) {
-    constexpr int i = decltype(i_c)::value;
-    if (i + N - 1 < left) load(st[(i + N - 1) % N]);
-    if (i < left) multiply(st[i % N]);
+};
+
+// One token or a few whose h fits LDS: grid H / 16, a block makes 16 columns of every token's row.  The waves put their partial
+// sums side by side in LDS and the block adds them up.  Four steps of loads in flight.
+template <class W, class X>
+__device__ void down_few_kernel(const MoeArgs& a, float* partial) {
+  __shared__ SortLds s;
+  __shared__ int spot[MOE_FEW * MOE_K];              // where a pair stands in the order of experts
+  __shared__ float picked[MOE_FEW * MOE_K], prob[MOE_FEW * MOE_K];
+  constexpr int NT = DOWN_WAVES * 64;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int pairs = a.T * a.k;                       // (at most as many as threads; experts at most half of that)
+  const int expert[1] = {tid < pairs ? a.ids[tid] : 0};
+  const float my_value = tid < pairs ? a.picked[tid] : 0.f;
+  // LDS behind the partial sums: h, upper parts, then lower ones, rows 8 values longer than they are (other banks).  The
+  // workspace holds the two planes side by side, pairs * I values each (I a multiple of 16): copied 16 bytes at a time.
+  constexpr int H_CHUNKS = MOE_H_LDS / 16 / NT;
+  const int per_row = a.I / 8, chunks = 2 * pairs * per_row, h_row = a.I + 8;
+  u32x4 hv[H_CHUNKS];
+#pragma unroll
+  for (int i = 0; i < H_CHUNKS; ++i) hv[i] = ((const u32x4_a*)a.h_hi)[min(tid + i * NT, chunks - 1)];
+  if (tid < pairs) picked[tid] = my_value;
+  sort_pairs<NT>(a, s, expert, [&](int pair, int at) { spot[pair] = at; });
+  const int parts = max(1, min(DOWN_WAVES / s.items, (a.I + GROUP - 1) / GROUP));
+  __bf16* h_lds = (__bf16*)(partial + pairs * parts * 16);
+  DownWave<W, 1, 4, true> d(a, s, h_lds, blockIdx.x * 16, parts, wave, DOWN_WAVES);
+#pragma unroll
+  for (int i = 0; i < H_CHUNKS; ++i) {
+    const int c = tid + i * NT, row = c / per_row;
+    if (c < chunks) *(u32x4_a*)(h_lds + row * h_row + (c - row * per_row) * 8) = hv[i];
+  }
+  if (tid < pairs) {
+    prob[tid] = pair_weight(a, picked + tid / a.k * a.k, tid % a.k);
+    if (blockIdx.x == 0) a.probs[tid] = prob[tid];
+  }
+  __syncthreads();
+  d.run([&](int which, int part, int, const f32x4& sum) {
+    if (d.r < s.item_count[which]) *(f32x4*)(partial + (((s.item_first[which] + d.r) * parts + part) * 16 + d.g * 4)) = sum;
   });
   __syncthreads();
-  for (int i = tid; i < a.T * 16; i += DOWN_WAVES * 64) {
+  for (int i = tid; i < a.T * 16; i += NT) {
     const int t = i >> 4, c = i & 15;
     float sum = 0.f;
 #pragma unroll 4
     for (int j = 0; j < a.k; ++j) {
-      const float p = s.prob[t * a.k + j];
-      const float* v = partial + s.spot[t * a.k + j] * parts * 16 + c;
+      const float p = prob[t * a.k + j];
+      const float* v = partial + spot[t * a.k + j] * parts * 16 + c;
       float y = 0.f;
       for (int q = 0; q < parts; ++q) y += v[q * 16];
       if (p != 0.f) sum = fmaf(p, y, sum);           // (a weight of 0 adds nothing, not even 0 * infinity)
     }
     ((X*)a.out)[(int64_t)t * a.out_stride + blockIdx.x * 16 + c] = (X)sum;
   }
+}
+
+// More of them: grid (H / 64, z), a block makes 64 columns of the pairs of its share of the items, which go to memory as
+// y[part][pair][H] in 32 bits; combine_kernel adds them up.  Four tiles beside each other use a load of h four times: with one
+// (and all items in one block, no memory between) the loads' addresses took longer than the weights.
+template <class W>
+__device__ void down_many_kernel(const MoeArgs& a) {
+  __shared__ SortLds s;
+  constexpr int NT = DOWN_MANY_WAVES * 64;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), pairs = a.T * a.k;
+  int expert[MOE_T * MOE_K / NT];
+#pragma unroll
+  for (int i = 0; i < MOE_T * MOE_K / NT; ++i) expert[i] = tid + i * NT < pairs ? a.ids[tid + i * NT] : 0;
+  sort_pairs<NT>(a, s, expert, [](int, int) {});
+  const int waves = gridDim.y * DOWN_MANY_WAVES;
+  const int parts = max(1, min(waves / s.items, a.max_parts));
+  if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *a.parts = parts;
+  const int n0 = blockIdx.x * DOWN_MANY_COLS;
+  DownWave<W, DOWN_MANY_COLS / 16, 2, false> d(a, s, nullptr, n0, parts, wave * gridDim.y + blockIdx.y, waves);
+  d.run([&](int which, int part, int t, const f32x4& sum) {
+    if (d.r < s.item_count[which] && n0 + t * 16 < a.H)
+      *(f32x4*)(a.y + ((int64_t)part * pairs + s.pair[s.item_first[which] + d.r]) * a.H + n0 + t * 16 + d.g * 4) = sum;
+  });
+}
+
+// out[t, c] = sum over places of their weight times the sum over parts; grid (H / 1024, T), four columns a thread
+template <class X>
+__device__ void combine_kernel(const MoeArgs& a) {
+  __shared__ float weight[MOE_K];
+  const int tid = threadIdx.x, t = blockIdx.y, c = (blockIdx.x * 256 + tid) * 4;
+  const int parts = *a.parts;
+  if (tid < a.k) {
+    weight[tid] = pair_weight(a, a.picked + t * a.k, tid);
+    if (blockIdx.x == 0) a.probs[t * a.k + tid] = weight[tid];
+  }
+  __syncthreads();
+  if (c >= a.H) return;
+  const int64_t plane = (int64_t)a.T * a.k * a.H;
+  const float* v = a.y + (int64_t)t * a.k * a.H + c;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](int j, const f32x4& y) {
+    const float p = weight[j];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = p != 0.f ? fmaf(p, y[i], sum[i]) : sum[i];      // (a weight of 0 adds nothing, not even 0 * infinity)
+  };
+  if (parts == 1) {
+#pragma unroll 8
+    for (int j = 0; j < a.k; ++j) add(j, *(const f32x4*)(v + (int64_t)j * a.H));
+  } else {
+    for (int j = 0; j < a.k; ++j) {
+      f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int q = 0; q < parts; ++q) y += *(const f32x4*)(v + (int64_t)j * a.H + q * plane);
+      add(j, y);
+    }
+  }
+  X* o = (X*)a.out + (int64_t)t * a.out_stride + c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = (X)sum[i];
 }
 
 }  // namespace kcg_ops
