@@ -7,6 +7,11 @@ exit status.
 
     python -m codegendemo_amd.kcg.test [case_normal_0 | case_normal_1 | case_bad_0]
     python -m codegendemo_amd.kcg.test --config TunedConfigs/gemm_4096_fp16.json --index 0 [--count 20]
+
+The operators of the 8-bit path, which take their sizes at run time, are checked the same way against their formulas in
+torch (an addition):
+
+    python -m codegendemo_amd.kcg.test --operator matmul_fp8 [--sizes 512 4096 4096] [--count 20]
 """
 import argparse
 import json
@@ -120,14 +125,117 @@ def test_correctness(kpm: KernelArgMatmul, deviceId: int = 0, benchmarkCount: in
     return ok
 
 
+# operator -> its sizes when --sizes does not give them
+OPERATORS = {"rmsnorm_quant": (1024, 4096),               # rows, columns
+             "swiglu_quant": (1024, 4096),                # rows, columns of the result
+             "matmul_fp8": (512, 4096, 4096),             # M, N, K
+             "moe_layer": (8, 32, 4, 2048, 1024)}         # tokens, experts, experts of a token, H, I
+
+
+def _widened(q, scale, blocks=False):
+    """e4m3 values and their scales (of 128 along a row, or of 128 x 128) as float32."""
+    s = scale.repeat_interleave(128, -1)[..., :q.shape[-1]]
+    return q.float() * (s.repeat_interleave(128, -2)[..., :q.shape[-2], :] if blocks else s)
+
+
+def _operator_case(name, sizes, dev, gen):
+    """(the operator's call, its formula in torch; both return one float32 tensor, the step of the result's type)"""
+    import torch
+    from .Operators.matmul_fp8 import matmul_fp8
+    from .Operators.moe import moe_layer
+    from .Operators.quant import rmsnorm_quant, swiglu_quant
+
+    def normal(*shape, std=1.0):
+        return torch.randn(*shape, dtype=torch.float32, device=dev, generator=gen) * std
+
+    def weight(*shape):
+        """e4m3 weights of values below 1, and a scale for each 128 x 128"""
+        w = normal(*shape).clamp_(-4, 4).mul_(100).to(torch.float8_e4m3fn)
+        return w, torch.full((*shape[:-2], -(-shape[-2] // 128), -(-shape[-1] // 128)), shape[-1] ** -0.5 / 100, device=dev)
+
+    silu = torch.nn.functional.silu
+    if name == "rmsnorm_quant":
+        x, w = normal(*sizes).bfloat16(), (1 + normal(sizes[1], std=0.1)).bfloat16()
+        return (lambda: _widened(*rmsnorm_quant(x, w)[:2]),
+                lambda: x.float() * torch.rsqrt(x.float().square().mean(1, keepdim=True) + 1e-6) * w.float(), 2.0 ** -4)
+    if name == "swiglu_quant":
+        t, i = sizes
+        x = normal(t, 2 * i).bfloat16()
+        return lambda: _widened(*swiglu_quant(x)), lambda: silu(x[:, :i].float()) * x[:, i:].float(), 2.0 ** -4
+    if name == "matmul_fp8":
+        m, n, k = sizes
+        k16 = -(-k // 16) * 16                             # rows start on 16 bytes
+        a, sa = normal(m, k16).clamp_(-4, 4).mul_(100).to(torch.float8_e4m3fn)[:, :k], torch.rand(m, -(-k // 128), device=dev, generator=gen) / 100
+        b, sb = weight(n, k16)
+        b = b[:, :k]
+        return lambda: matmul_fp8(a, sa, b, sb).float(), lambda: _widened(a, sa) @ _widened(b, sb, True).t(), 2.0 ** -8
+    t, e, k, h, i = sizes
+    x, logits = normal(t, h).bfloat16(), normal(t, e)
+    (w13, s13), (w2, s2) = weight(e, 2 * i, h), weight(e, h, i)
+
+    def formula():
+        p, ids = torch.sort(logits, dim=1, descending=True, stable=True)
+        p, ids = torch.softmax(p[:, :k], 1), ids[:, :k]
+        out = torch.zeros(t, h, device=dev)
+        for token in range(t):
+            for place in range(k):
+                j = int(ids[token, place])
+                gate_up = _widened(w13[j], s13[j], True) @ x[token].float()
+                out[token] += p[token, place] * (_widened(w2[j], s2[j], True) @ (silu(gate_up[:i]) * gate_up[i:]))
+        return out
+    return lambda: moe_layer(x, logits, k, w13, w2, s13, s2)[0].float(), formula, 2.0 ** -8
+
+
+def test_operator(name: str, sizes=None, deviceId: int = 0, benchmarkCount: int = 1, seed: int = 0x4B4347) -> bool:
+    """One operator of the 8-bit path on seeded inputs against its formula: within a step of the result's type, and 1/1000 of
+    the largest result for what sums lose and for the smallest 8-bit values."""
+    import torch
+    sizes = tuple(sizes or OPERATORS[name])
+    dev = torch.device("cuda", deviceId)
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(seed)
+    call, formula, step = _operator_case(name, sizes, dev, gen)
+    print("===== test info ========")
+    print(f"operator =  {name}, sizes =  {sizes}")
+
+    def timed(f):
+        times, result = [], None
+        for _ in range(max(1, benchmarkCount)):
+            torch.cuda.synchronize(dev)
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record(torch.cuda.current_stream(dev))
+            result = f()
+            end.record(torch.cuda.current_stream(dev))
+            torch.cuda.synchronize(dev)
+            times.append(start.elapsed_time(end))
+        return result, float(np.median(times))
+
+    got, ms = timed(call)
+    want, plain_ms = timed(formula)
+    print(f"codegenDemo median time: {ms} ms")
+    print(f"torch median time: {plain_ms} ms")
+    off = (got - want).abs()
+    ok = bool((off <= want.abs() * step + want.abs().max() * 1e-3).all())
+    print('test correct!' if ok else f'test fail! maxerror={off.max().item()}')
+    return ok
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description="single-config check against the library GEMM")
     ap.add_argument("case", nargs="?", default="case_normal_0", choices=sorted(CASES))
+    ap.add_argument("--operator", choices=sorted(OPERATORS), help="check an operator of the 8-bit path instead of a config")
+    ap.add_argument("--sizes", type=int, nargs="+", help="the operator's sizes")
     ap.add_argument("--config", help="JSON file: {\"cfgs\": [...]}, {\"results\": [{\"config\": ...}]} or one flat config")
     ap.add_argument("--index", type=int, default=0)
     ap.add_argument("--count", type=int, default=1, help="timed runs of each side (the reference uses 1)")
     ap.add_argument("--device", type=int, default=0)
     args = ap.parse_args(argv)
+    if args.sizes and not args.operator:
+        ap.error("--sizes goes with --operator")
+    if args.operator:
+        if args.sizes and (len(args.sizes) != len(OPERATORS[args.operator]) or min(args.sizes) < 1):
+            ap.error(f"{args.operator} takes {len(OPERATORS[args.operator])} positive sizes")
+        return 0 if test_operator(args.operator, args.sizes, args.device, args.count) else 1
     if args.config:
         with open(args.config) as f:
             obj = json.load(f)

@@ -482,3 +482,12 @@ def test_norm_of_rows_whose_squares_leave_the_range(h, dtype, size):
         want = R.norm64(x, None, w, eps)[1]
         assert bool(((y.double() - want).abs() <= want.abs() * (R.half_step(dtype) + R.NORM_REL) + R.smallest(dtype)).all())
         R.check_quantized(q, s, want, R.NORM_REL)
+
+
+@pytest.mark.parametrize("operator,sizes", [("rmsnorm_quant", None), ("swiglu_quant", ["33", "1000"]), ("matmul_fp8", ["100", "333", "450"]), ("moe_layer", None)])
+def test_operator_check_command(operator, sizes, capsys):
+    """python -m codegendemo_amd.kcg.test --operator <name> [--sizes ...]"""
+    from codegendemo_amd.kcg import test as single
+    print(f"[case] operator check {operator}", flush=True)
+    assert single.main(["--operator", operator] + (["--sizes", *sizes] if sizes else [])) == 0
+    assert "test correct!" in capsys.readouterr().out

@@ -156,3 +156,11 @@ def test_the_tested_products_reach_every_kernel():
     assert all(_native_ops.matmul_fp8_kernel(m, n, k, BF16) for m, n, k, _ in MATMULS)
     with pytest.raises(_native.KcgError):
         _native_ops.matmul_fp8_kernel(1, 1, 1, F64)
+
+
+@pytest.mark.parametrize("argv", [["--operator", "matmul_fp8", "--sizes", "1", "2"], ["--operator", "swiglu_quant", "--sizes", "0", "4"], ["--sizes", "4"], ["--operator", "softmax"]])
+def test_operator_check_command_refuses(argv, capsys):
+    from codegendemo_amd.kcg import test as single
+    with pytest.raises(SystemExit) as e:
+        single.main(argv)
+    assert e.value.code == 2 and "error" in capsys.readouterr().err
