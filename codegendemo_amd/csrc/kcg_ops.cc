@@ -240,6 +240,7 @@ int type_index(int64_t dtype) { return dtype == KCG_DT_BFLOAT16 ? 0 : dtype == K
 int type_bytes(int64_t dtype) { return dtype == KCG_DT_FLOAT32 ? 4 : dtype == KCG_DT_E4M3 ? 1 : 2; }
 constexpr int64_t kMaxExtent = 1 << 30;       // rows and columns: 32-bit indices in the kernels, with room for a tile
 constexpr int64_t kMaxStride = (int64_t)1 << 40;
+constexpr int64_t kMaxThreads = UINT_MAX;     // of a launch
 bool extent_ok(int64_t n) { return n >= 0 && n <= kMaxExtent; }
 // a row stride: rows do not overlap (any value goes where there is one row)
 bool stride_ok(int64_t stride, int64_t cols, int64_t rows) { return stride >= 0 && stride <= kMaxStride && (rows <= 1 || stride >= cols); }
@@ -290,6 +291,7 @@ int kcg_rmsnorm_quant(const kcg_rmsnorm_quant_args* p, int device, uint64_t stre
   const int v = nv <= 64 ? 0 : nv <= 128 ? 1 : nv <= 256 ? 2 : nv <= 512 ? 3 : nv <= 1024 ? 4 : nv <= 2048 ? 5 : 6;
   static const int threads[7] = {256, 128, 256, 512, 1024, 1024, 1024};
   const int64_t blocks = v == 0 ? (p->rows + 3) / 4 : p->rows;
+  if (blocks * threads[v] > kMaxThreads) return bad("rmsnorm_quant: rows * cols is too large");
   return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) {
     return launch(hip, k.fn[kNorm + t * 7 + v], (unsigned)blocks, 1, threads[v], 0, stream, &a);
   });
@@ -308,7 +310,7 @@ int kcg_swiglu_quant(const kcg_swiglu_quant_args* p, int device, uint64_t stream
     return bad("swiglu_quant: a row stride is negative or smaller than a row");
   if (!scale_layout_ok(p->scale_stride_row, p->scale_stride_group, p->rows, groups(p->cols))) return bad("swiglu_quant: scales overlap");
   const int64_t threads = p->rows * groups(p->cols) * 16;
-  if (threads > (int64_t)UINT_MAX - 256) return bad("swiglu_quant: rows * cols is too large");
+  if (threads > kMaxThreads - 256) return bad("swiglu_quant: rows * cols is too large");
   SwigluArgs a = {(const void*)p->gate_up, (uint8_t*)p->q, (float*)p->scale, p->gate_up_stride, p->q_stride, p->scale_stride_row, p->scale_stride_group,
                   (unsigned)p->rows, (int)p->cols};
   return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) {
@@ -341,7 +343,7 @@ int kcg_matmul_fp8(const kcg_matmul_fp8_args* p, int device, uint64_t stream) {
                   p->b_scale_stride_row, p->b_scale_stride_group, (int)p->m, (int)p->n, (int)p->k, (int)groups(p->k), 0, 0, 0};
   a.c_wide = aligned(p->c, 4 * es) && (p->m == 1 || aligned(p->c_stride, 4));
   const MatmulChoice c = choose_matmul(p->m, p->n, p->k, t);
-  if (c.blocks > (1 << 30)) return bad("matmul_fp8: m * n is too large");
+  if (c.blocks * c.threads > kMaxThreads) return bad("matmul_fp8: m * n is too large");
   a.grid_m = c.grid_m;
   a.grid_n = c.grid_n;
   return on_device(device, [&](const HostHip* hip, const DeviceKernels& k) { return launch(hip, k.fn[c.fn], (unsigned)c.blocks, 1, c.threads, 0, stream, &a); });

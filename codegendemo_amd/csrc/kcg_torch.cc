@@ -120,7 +120,11 @@ bool run(int (*entry)(const Args*, int, uint64_t), const Args& args, int device)
   const uint64_t stream = handle ? PyLong_AsUnsignedLongLongMask(handle) : 0;
   Py_XDECREF(handle);
   if (!handle || PyErr_Occurred()) return false;
-  const int status = entry(&args, device, stream);
+  TORCH_CHECK(entry, "_kcg_torch is not bound to the library: call the operators through codegendemo_amd.kcg.Operators");
+  int status;
+  Py_BEGIN_ALLOW_THREADS                     // (a launch waits where the device's queue is full)
+  status = entry(&args, device, stream);
+  Py_END_ALLOW_THREADS
   if (status >= 0) return true;
   PyObject* r = PyObject_CallFunction(check_status, "i", status);      // raises
   Py_XDECREF(r);

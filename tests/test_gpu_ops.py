@@ -423,6 +423,42 @@ def test_two_runs_give_the_same_bits():
         assert torch.equal(moe_layer(x, logits, 4, w13, w2, s13, s2)[0], first[0]) and torch.equal(matmul_fp8(a, sa, b, sb), first[1])
 
 
+def test_calls_of_two_threads_on_streams_of_their_own():
+    import threading
+    g = gen(13)
+    w13, w2, s13, s2 = experts(g, 16, 512, 256, E4M3)
+    b, sb = to8(torch.randn(700, 512, device=DEV, generator=g), 128)
+    inputs = [(torch.randn(t, 512, device=DEV, generator=g).to(BF16), torch.randn(t, 16, device=DEV, generator=g)) for t in (1, 23)]
+    norm_w = torch.ones(512, dtype=BF16, device=DEV)
+
+    def step(x, logits):
+        q, s, y, _ = rmsnorm_quant(x, norm_w, want_y=True)
+        return matmul_fp8(q, s, b, sb), moe_layer(y, logits, 4, w13, w2, s13, s2)[0]
+
+    want = [step(*i) for i in inputs]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def worker(n):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(30):
+                    got[n].append(step(*inputs[n]))
+            stream.synchronize()
+        except Exception as e:      # reported by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=worker, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for n in range(2):
+        assert all(torch.equal(a, w) for out in got[n] for a, w in zip(out, want[n]))
+
+
 def test_empty_tensors():
     q, s, y, r = rmsnorm_quant(torch.empty(0, 64, dtype=BF16, device=DEV), torch.ones(64, dtype=BF16, device=DEV))
     assert q.shape == (0, 64) and s.shape == (0, 1)

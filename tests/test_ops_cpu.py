@@ -73,7 +73,8 @@ BAD = [
     ("kcg_swiglu_quant", dict(dtype=F64), "bfloat16, float16 or float32"), ("kcg_swiglu_quant", dict(cols=-1), "rows and cols"), ("kcg_swiglu_quant", dict(gate_up=0), "null"),
     ("kcg_swiglu_quant", dict(gate_up=P + 1), "aligned"), ("kcg_swiglu_quant", dict(q=P + 4), "16 bytes"), ("kcg_swiglu_quant", dict(q_stride=248), "16 bytes"),
     ("kcg_swiglu_quant", dict(gate_up_stride=-1), "row stride"), ("kcg_swiglu_quant", dict(q_stride=16), "row stride"), ("kcg_swiglu_quant", dict(scale_stride_row=1), "overlap"),
-    ("kcg_swiglu_quant", dict(rows=1 << 28, q_stride=256), "too large"),
+    ("kcg_swiglu_quant", dict(rows=1 << 28, q_stride=256), "too large"), ("kcg_rmsnorm_quant", dict(rows=1 << 28), "too large"),
+    ("kcg_matmul_fp8", dict(m=1 << 30, n=1 << 30, c_stride=1 << 30), "too large"),
     ("kcg_matmul_fp8", dict(c_dtype=F64), "bfloat16, float16 or float32"), ("kcg_matmul_fp8", dict(m=-1), "m, n and k"), ("kcg_matmul_fp8", dict(k=(1 << 30) + 1), "m, n and k"),
     ("kcg_matmul_fp8", dict(a=0), "null"), ("kcg_matmul_fp8", dict(b_scale=0), "null"), ("kcg_matmul_fp8", dict(c=0), "null"), ("kcg_matmul_fp8", dict(c=P + 2), "aligned"),
     ("kcg_matmul_fp8", dict(a_scale=P + 1), "aligned"), ("kcg_matmul_fp8", dict(a=P + 8), "16 bytes"), ("kcg_matmul_fp8", dict(b_stride=200), "16 bytes"),
