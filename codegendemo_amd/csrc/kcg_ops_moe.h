@@ -613,31 +613,31 @@ __device__ void combine_kernel(const MoeArgs& a) {
   __shared__ float weight[MOE_K];
   const int tid = threadIdx.x, t = blockIdx.y, c = (blockIdx.x * 256 + tid) * 4;
   const int parts = *a.parts;
+  const int64_t plane = (int64_t)a.T * a.k * a.H;
+  const float* v = a.y + (int64_t)t * a.k * a.H + min(c, a.H - 4);
+  // (the first parts of the first places are on their way before the weights are there)
+  constexpr int AHEAD = 8;
+  f32x4 ahead[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) ahead[j] = *(const f32x4*)(v + (int64_t)min(j, a.k - 1) * a.H);
   if (tid < a.k) {
     weight[tid] = pair_weight(a, a.picked + t * a.k, tid);
     if (blockIdx.x == 0) a.probs[t * a.k + tid] = weight[tid];
   }
   __syncthreads();
   if (c >= a.H) return;
-  const int64_t plane = (int64_t)a.T * a.k * a.H;
-  const float* v = a.y + (int64_t)t * a.k * a.H + c;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  auto add = [&](int j, const f32x4& y) {
+  auto add = [&](int j, f32x4 y) {
+#pragma unroll 4
+    for (int q = 1; q < parts; ++q) y += *(const f32x4*)(v + (int64_t)j * a.H + q * plane);
     const float p = weight[j];
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum[i] = p != 0.f ? fmaf(p, y[i], sum[i]) : sum[i];      // (a weight of 0 adds nothing, not even 0 * infinity)
   };
-  if (parts == 1) {
-#pragma unroll 8
-    for (int j = 0; j < a.k; ++j) add(j, *(const f32x4*)(v + (int64_t)j * a.H));
-  } else {
-    for (int j = 0; j < a.k; ++j) {
-      f32x4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int q = 0; q < parts; ++q) y += *(const f32x4*)(v + (int64_t)j * a.H + q * plane);
-      add(j, y);
-    }
-  }
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (j < a.k) add(j, ahead[j]);
+  for (int j = AHEAD; j < a.k; ++j) add(j, *(const f32x4*)(v + (int64_t)j * a.H));
   X* o = (X*)a.out + (int64_t)t * a.out_stride + c;
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = (X)sum[i];
