@@ -1,8 +1,7 @@
 """ctypes binding of the operators of the 8-bit path in libkcg_gemm.so (C ABI: include/kcg_ops.h).
 
-A call's arguments travel as one packed block (all fields are 64 bits wide), which costs a launch about a microsecond of
-host time where a ctypes argument for each field would cost several.  The three small operators are called on torch tensors
-through a compiled module of their own (csrc/kcg_torch.cc), which this one hands the library's entry points."""
+A call's arguments travel as one packed block (all fields are 64 bits wide), in the order of the header's structs.  On torch tensors
+the operators are called through a compiled module (csrc/kcg_torch.cc), which this one hands the library's entry points."""
 import ctypes
 import importlib
 import os
@@ -50,7 +49,7 @@ def torch_ops():
         except ImportError as e:
             raise ImportError(f"{os.path.join(os.path.dirname(_native.LIB_PATH), '_kcg_torch.so')}: {e}; build it again for this torch "
                               f"(`make -C {_native.CSRC_DIR}` or __graft_entry__.build())") from e
-        entries = [ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in ("kcg_rmsnorm_quant", "kcg_swiglu_quant", "kcg_matmul_fp8")]
+        entries = [ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in ("kcg_rmsnorm_quant", "kcg_swiglu_quant", "kcg_matmul_fp8", "kcg_moe_layer", "kcg_moe_workspace_bytes")]
         m.bind(*entries, torch._C._cuda_getCurrentRawStream, _native.check)
         _torch_ops = m
     return _torch_ops

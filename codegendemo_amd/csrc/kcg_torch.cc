@@ -1,7 +1,7 @@
-// kcg_torch.cc — the small operators of the 8-bit path on torch tensors: checks of the arguments, outputs, the call.
-// A call of theirs is over in 3 to 5 us on the GPU, and the runtime's launch takes the host 3.1; with the same steps in Python a
+// kcg_torch.cc — the operators of the 8-bit path on torch tensors: checks of the arguments, outputs, the call.
+// A small call is over in 3 to 5 us on the GPU, and the runtime's launch takes the host 3.1; with the same steps in Python a
 // call took the host 7.4 to 8.5 us (an output 1.3, a checked operand 0.5), so a decoded token waited for it.  Here a whole call
-// takes 4.3 to 4.7 us.
+// takes 4.3 to 4.7 us (moe_layer, of two or three launches: 8.5, 11).
 //
 // The module links neither the library nor a HIP runtime: bind() gives it the addresses of the C entry points
 // (include/kcg_ops.h), so that both bindings run the one library that the process has loaded.
@@ -22,6 +22,8 @@ using at::ScalarType;
 int (*norm_entry)(const kcg_rmsnorm_quant_args*, int, uint64_t);
 int (*swiglu_entry)(const kcg_swiglu_quant_args*, int, uint64_t);
 int (*matmul_entry)(const kcg_matmul_fp8_args*, int, uint64_t);
+int (*moe_entry)(const kcg_moe_layer_args*, int, uint64_t);
+int64_t (*moe_workspace)(int64_t, int64_t, int64_t, int64_t, int64_t);
 PyObject* stream_of;       // device index -> raw handle of torch's current stream
 PyObject* check_status;    // raises what a negative status stands for
 
@@ -111,6 +113,13 @@ struct Matrix {
 
 int64_t ld16(int64_t cols) { return (cols + 15) / 16 * 16; }
 
+// raises what a negative status stands for
+void raise_status(int status) {
+  PyObject* r = PyObject_CallFunction(check_status, "i", status);
+  Py_XDECREF(r);
+  if (r) PyErr_Format(PyExc_RuntimeError, "status %d", status);
+}
+
 // false: a Python error is set
 template <class Args>
 bool run(int (*entry)(const Args*, int, uint64_t), const Args& args, int device) {
@@ -126,9 +135,7 @@ bool run(int (*entry)(const Args*, int, uint64_t), const Args& args, int device)
   status = entry(&args, device, stream);
   Py_END_ALLOW_THREADS
   if (status >= 0) return true;
-  PyObject* r = PyObject_CallFunction(check_status, "i", status);      // raises
-  Py_XDECREF(r);
-  if (r) PyErr_Format(PyExc_RuntimeError, "status %d", status);
+  raise_status(status);
   return false;
 }
 
@@ -139,16 +146,19 @@ bool count(const char* name, Py_ssize_t n, Py_ssize_t want) {
 }
 
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!count("bind", n, 5)) return nullptr;
-  const uint64_t entries[3] = {PyLong_AsUnsignedLongLong(a[0]), PyLong_AsUnsignedLongLong(a[1]), PyLong_AsUnsignedLongLong(a[2])};
+  if (!count("bind", n, 7)) return nullptr;
+  uint64_t entries[5];
+  for (int i = 0; i < 5; ++i) entries[i] = PyLong_AsUnsignedLongLong(a[i]);
   if (PyErr_Occurred()) return nullptr;
   norm_entry = (decltype(norm_entry))(uintptr_t)entries[0];
   swiglu_entry = (decltype(swiglu_entry))(uintptr_t)entries[1];
   matmul_entry = (decltype(matmul_entry))(uintptr_t)entries[2];
+  moe_entry = (decltype(moe_entry))(uintptr_t)entries[3];
+  moe_workspace = (decltype(moe_workspace))(uintptr_t)entries[4];
   Py_XDECREF(stream_of);
   Py_XDECREF(check_status);
-  stream_of = Py_NewRef(a[3]);
-  check_status = Py_NewRef(a[4]);
+  stream_of = Py_NewRef(a[5]);
+  check_status = Py_NewRef(a[6]);
   Py_RETURN_NONE;
 }
 
@@ -272,9 +282,90 @@ PyObject* matmul_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// weights [experts, rows, cols] with contiguous rows
+void check_experts(const char* name, const at::Tensor& t, int64_t experts, int64_t rows, int64_t cols, at::Device device) {
+  TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.device() == device && t.dim() == 3 && t.size(0) == experts && t.size(1) == rows && t.size(2) == cols, name,
+                    " must have shape (", experts, ", ", rows, ", ", cols, ") on ", device.str(), ", got ", t.sizes(), " on ", t.device().str());
+  TORCH_CHECK_VALUE(t.stride(2) == 1 || cols <= 1, name, ": the elements of a row must lie side by side, got strides ", t.strides());
+}
+
+// contiguous scales of blocks of 128 x 128 of `w`
+int64_t block_scales(const char* name, PyObject* o, const at::Tensor& w, at::Device device) {
+  const at::Tensor* s = o == Py_None ? nullptr : &tensor(name, o);
+  const int64_t e = w.size(0), r = groups(w.size(1)), c = groups(w.size(2));
+  TORCH_CHECK_VALUE(s && s->scalar_type() == ScalarType::Float && s->device() == device && s->dim() == 3 && s->size(0) == e && s->size(1) == r &&
+                        s->size(2) == c && s->is_contiguous(),
+                    name, " must be a contiguous torch.float32 tensor of shape (", e, ", ", r, ", ", c, ") on ", device.str());
+  return address(*s);
+}
+
+// (x, logits, topk, w13, w2, w13_scale, w2_scale, renormalize, out) -> (out, ids, probs)
+PyObject* moe_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!count("moe_layer", n, 9)) return nullptr;
+  const at::Tensor &x = tensor("x", a[0]), &logits = tensor("logits", a[1]), &w13 = tensor("w13", a[3]), &w2 = tensor("w2", a[4]);
+  on_gpu("x", x);
+  TORCH_CHECK_VALUE(x.dim() == 2 && logits.dim() == 2 && w13.dim() == 3, "x and logits must be matrices, w13 and w2 [experts, rows, columns]");
+  const at::Device device = x.device();
+  const ScalarType type = x.scalar_type(), wt = w13.scalar_type();
+  kcg_moe_layer_args p = {};
+  p.tokens = x.size(0);
+  p.hidden = x.size(1);
+  p.experts = logits.size(1);
+  p.topk = PyLong_AsLongLong(a[2]);
+  const int renormalize = PyObject_IsTrue(a[7]);
+  if (PyErr_Occurred()) return nullptr;
+  p.renormalize = renormalize;
+  TORCH_CHECK_VALUE(w13.size(1) % 2 == 0, "w13 holds two weights of the same number of rows, got ", w13.size(1), " rows");
+  p.inter = w13.size(1) / 2;
+  p.x_stride = matrix("x", x, p.tokens, p.hidden, type, device);
+  p.logits_stride = matrix("logits", logits, p.tokens, p.experts, ScalarType::Float, device);
+  check_experts("w13", w13, p.experts, 2 * p.inter, p.hidden, device);
+  check_experts("w2", w2, p.experts, p.hidden, p.inter, device);
+  TORCH_CHECK_TYPE(w2.scalar_type() == wt && (wt == ScalarType::Float8_e4m3fn || wt == ScalarType::BFloat16) &&
+                       (type == ScalarType::BFloat16 || type == ScalarType::Half),
+                   "weights of ", c10::toString(wt), " and ", c10::toString(w2.scalar_type()), " with x of ", c10::toString(type),
+                   ": e4m3 weights take bfloat16 or float16, bfloat16 weights bfloat16");
+  if (wt == ScalarType::Float8_e4m3fn) {
+    p.w13_scale = block_scales("w13_scale", a[5], w13, device);
+    p.w2_scale = block_scales("w2_scale", a[6], w2, device);
+    p.weight_dtype = KCG_DT_E4M3;
+  } else {
+    TORCH_CHECK_VALUE(a[5] == Py_None && a[6] == Py_None, "bfloat16 weights have no scales");
+    p.weight_dtype = KCG_DT_BFLOAT16;
+  }
+  p.dtype = code_of(type);
+  TORCH_CHECK(moe_workspace, "_kcg_torch is not bound to the library: call the operators through codegendemo_amd.kcg.Operators");
+  p.workspace_bytes = moe_workspace(p.tokens, p.experts, p.topk, p.hidden, p.inter);
+  if (p.workspace_bytes < 0) {
+    raise_status((int)p.workspace_bytes);
+    return nullptr;
+  }
+  Matrix out, ids, probs;
+  out.output("out", a[8], p.tokens, p.hidden, p.hidden, type, device);
+  ids.made(p.tokens, p.topk, p.topk, ScalarType::Int, device);
+  probs.made(p.tokens, p.topk, p.topk, ScalarType::Float, device);
+  p.x = address(x), p.logits = address(logits), p.w13 = address(w13), p.w2 = address(w2);
+  p.out = out.address, p.out_stride = out.row, p.ids = ids.address, p.probs = probs.address;
+  p.w13_stride_expert = w13.stride(0), p.w13_stride_row = w13.stride(1), p.w2_stride_expert = w2.stride(0), p.w2_stride_row = w2.stride(1);
+  if (p.tokens) {
+    // (freed to torch's allocator on return: what takes it over runs behind this call on the same stream)
+    const at::Tensor workspace = at::empty_strided({p.workspace_bytes}, {1}, at::TensorOptions().dtype(ScalarType::Byte).device(device));
+    p.workspace = address(workspace);
+    if (!run(moe_entry, p, device.index())) return nullptr;
+  }
+  PyObject* r = PyTuple_New(3);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, out.release());
+  PyTuple_SET_ITEM(r, 1, ids.release());
+  PyTuple_SET_ITEM(r, 2, probs.release());
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
 #define METHOD(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind), METHOD(rmsnorm_quant), METHOD(swiglu_quant), METHOD(matmul_fp8), {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kcg_torch", "The small operators of the 8-bit path on torch tensors.", -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyMethodDef methods[] = {METHOD(bind), METHOD(rmsnorm_quant), METHOD(swiglu_quant), METHOD(matmul_fp8), METHOD(moe_layer), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kcg_torch", "The operators of the 8-bit path on torch tensors.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 
