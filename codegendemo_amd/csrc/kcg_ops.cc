@@ -66,7 +66,7 @@ double skinny_estimate(int rt, int64_t n, int64_t groups) {
   return 2.2 + groups * (rt == 1 ? .172 : .24) * (rounds > 1 ? rounds : 1);
 }
 
-enum { kNorm = 0, kSwiglu = kNorm + 21, kSkinny = kSwiglu + 3, kTile = kSkinny + 12, kMoeUp = kTile + 3 * kTiles, kMoeFew = kMoeUp + 3, kMoeMany = kMoeFew + 3, kMoeCombine = kMoeMany + 2, kNumKernels = kMoeCombine + 2 };
+enum { kNorm = 0, kSwiglu = kNorm + 21, kSkinny = kSwiglu + 3, kTile = kSkinny + 12, kMoeUp = kTile + 3 * kTiles, kMoeFew = kMoeUp + 3, kMoeMany = kMoeFew + 3, kMoeCombine = kMoeMany + 4, kNumKernels = kMoeCombine + 2 };
 
 std::string kernel_symbol(int i) {
   static const char* const types[3] = {"bf16", "f16", "f32"};
@@ -81,7 +81,7 @@ std::string kernel_symbol(int i) {
   if (i < kMoeUp) return std::string("kcg_mm8_tile_") + types[(i - kTile) / kTiles] + "_" + kTileTable[(i - kTile) % kTiles].name;
   if (i < kMoeFew) return std::string("kcg_moe_up_") + moe[i - kMoeUp];
   if (i < kMoeMany) return std::string("kcg_moe_down_few_") + moe[i - kMoeFew];
-  if (i < kMoeCombine) return i == kMoeMany ? "kcg_moe_down_many_e4m3" : "kcg_moe_down_many_bf16";
+  if (i < kMoeCombine) return std::string("kcg_moe_down_many_") + ((i - kMoeMany) / 2 ? "bf16_" : "e4m3_") + ((i - kMoeMany) % 2 ? "16" : "8");
   return i == kMoeCombine ? "kcg_moe_combine_bf16" : "kcg_moe_combine_f16";
 }
 
@@ -153,7 +153,7 @@ int64_t groups(int64_t n) { return (n + 127) / 128; }
 struct MoePlan {
   int64_t slots, plane, parts_at, y_at, bytes;     // bytes of one plane of h; where the number of parts and y stand
   bool few;                                        // h fits LDS: one kernel for the second product and the sum
-  int z, max_parts;
+  int per, z, max_parts;                           // pairs an item holds, blocks that share the items, most parts of I
 };
 MoePlan moe_plan(int64_t tokens, int64_t experts, int64_t topk, int64_t hidden, int64_t inter) {
   MoePlan m = {};
@@ -164,9 +164,12 @@ MoePlan moe_plan(int64_t tokens, int64_t experts, int64_t topk, int64_t hidden, 
   // 4096 x 2048 in bf16: 63.7 us, the other way 50.5; 2 tokens, 8 of 128 experts of 1024 x 4096: 46.4, the other way 53)
   m.few = tokens <= MOE_FEW && moe_h_bytes(pairs, inter) <= (hidden >= 16 * 256 ? MOE_H_LDS : MOE_H_LDS / 2);
   // one block on each of the 256 compute units; waves without an item of their own share I, in parts.  There are at least
-  // `items` items: k experts, and 8 pairs an item.
+  // `items` items: k experts, and `per` pairs an item.
   m.z = cols >= 256 ? 1 : (int)(256 / cols);
-  const int64_t items = std::max<int64_t>(std::max<int64_t>(topk, (pairs + 7) / 8), 1);
+  // Items of 16 pairs halve the reads of W2 by experts of more than 8 tokens and cost the others four more loads a step: 64 tokens, 4 of 16
+  // experts of 2048 x 4096 48 us (by eight 57), 2 of 8 of 2048 x 4096 25 (27); 8 tokens an expert cost the same either way.
+  m.per = pairs > 8 * experts ? 16 : 8;
+  const int64_t items = std::max<int64_t>(std::max<int64_t>(topk, (pairs + m.per - 1) / m.per), 1);
   m.max_parts = (int)std::max<int64_t>(1, std::min<int64_t>(m.z * DOWN_MANY_WAVES / items, groups(inter)));
   m.parts_at = 2 * m.plane + pairs * 4;
   m.y_at = (m.parts_at + 4 + 15) / 16 * 16;
@@ -411,7 +414,7 @@ int kcg_moe_layer(const kcg_moe_layer_args* p, int device, uint64_t stream) {
     if (m.few)
       return launch(hip, k.fn[kMoeFew + v], (unsigned)(p->hidden / 16), 1, DOWN_WAVES * 64,
                     moe_partial_bytes(p->tokens) + (int)moe_h_bytes(p->tokens * p->topk, p->inter), stream, &a);
-    if (int rc = launch(hip, k.fn[kMoeMany + (v == 2)], (unsigned)((p->hidden + DOWN_MANY_COLS - 1) / DOWN_MANY_COLS), (unsigned)m.z, DOWN_MANY_WAVES * 64, 0,
+    if (int rc = launch(hip, k.fn[kMoeMany + 2 * (v == 2) + (m.per == 16)], (unsigned)((p->hidden + DOWN_MANY_COLS - 1) / DOWN_MANY_COLS), (unsigned)m.z, DOWN_MANY_WAVES * 64, 0,
                         stream, &a))
       return rc;
     return launch(hip, k.fn[kMoeCombine + (v == 1)], (unsigned)((p->hidden + 1023) / 1024), (unsigned)p->tokens, 256, 0, stream, &a);

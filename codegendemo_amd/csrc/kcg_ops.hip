@@ -54,7 +54,9 @@ MOE(Bf16Ops, uint8_t, __bf16, e4m3_bf16)
 MOE(F16Ops, uint8_t, _Float16, e4m3_f16)
 MOE(Bf16Ops, __bf16, __bf16, bf16_bf16)
 // (these keep nothing in x's type)
-extern "C" __global__ void __launch_bounds__(DOWN_MANY_WAVES * 64, 2) kcg_moe_down_many_e4m3(MoeArgs a) { down_many_kernel<uint8_t>(a); }
-extern "C" __global__ void __launch_bounds__(DOWN_MANY_WAVES * 64, 2) kcg_moe_down_many_bf16(MoeArgs a) { down_many_kernel<__bf16>(a); }
+#define DOWN_MANY(W, NAME, PER) \
+  extern "C" __global__ void __launch_bounds__(DOWN_MANY_WAVES * 64, 2) kcg_moe_down_many_##NAME##_##PER(MoeArgs a) { down_many_kernel<W, PER>(a); }
+DOWN_MANY(uint8_t, e4m3, 8) DOWN_MANY(uint8_t, e4m3, 16)
+DOWN_MANY(__bf16, bf16, 8) DOWN_MANY(__bf16, bf16, 16)
 extern "C" __global__ void __launch_bounds__(256) kcg_moe_combine_bf16(MoeArgs a) { combine_kernel<__bf16>(a); }
 extern "C" __global__ void __launch_bounds__(256) kcg_moe_combine_f16(MoeArgs a) { combine_kernel<_Float16>(a); }

@@ -340,12 +340,13 @@ __device__ void up_kernel(const MoeArgs& a) {
 
 // ---- down ----------------------------------------------------------------------------------------
 // Work items are (expert, up to 8 of its tokens): the 16 columns of a product hold the upper parts of 8 tokens' h and beside
-// them the lower ones, whose sums are added at the end, so that a group of 128 costs four loads of h and not eight.  Waves
-// take (item, part of I) in turn; sums over parts and over a token's places run in a fixed order.
+// them the lower ones, whose sums are added at the end, so that a group of 128 costs four loads of h and not eight.  Where
+// experts have more tokens an item holds 16 and takes the lower parts as a second product.  Waves take (item, part of I) in
+// turn; sums over parts and over a token's places run in a fixed order.
 struct SortLds {
   unsigned long long tokens[MOE_E];   // which tokens chose the expert
   int first[MOE_E];            // pairs of the experts in front of it
-  short item_expert[MOE_ITEMS], item_first[MOE_ITEMS], item_count[MOE_ITEMS];   // up to 8 pairs of one expert
+  short item_expert[MOE_ITEMS], item_first[MOE_ITEMS], item_count[MOE_ITEMS];   // up to 8 (16) pairs of one expert
   int pair[MOE_T * MOE_K];     // pairs (t k + place) by expert, then token
   int wave_sum[DOWN_WAVES];
   int items;
@@ -353,7 +354,7 @@ struct SortLds {
 
 // The pairs in the order of their experts, cut into items; NT >= MOE_E threads, thread i has the experts of pairs i, i + NT, ...
 // Ends with a barrier; at(pair, spot) is told where each pair stands.
-template <int NT, class F>
+template <int NT, int PER, class F>
 __device__ __forceinline__ void sort_pairs(const MoeArgs& a, SortLds& s, const int (&expert)[MOE_T * MOE_K / NT], F&& at_spot) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pairs = a.T * a.k;
   if (a.T == 1) {
@@ -376,7 +377,7 @@ __device__ __forceinline__ void sort_pairs(const MoeArgs& a, SortLds& s, const i
   __syncthreads();
   // the chosen experts' items side by side, and how many pairs lie in front of each expert
   const int n = tid < a.E ? __popcll(s.tokens[tid]) : 0;
-  const int mine = (n + 7) / 8;                    // items of this thread's expert
+  const int mine = (n + PER - 1) / PER;            // items of this thread's expert
   int upto = n << 16 | mine;                       // inclusive sums over the wave's lanes, of pairs (<= 1024) and items (<= 512)
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -391,8 +392,8 @@ __device__ __forceinline__ void sort_pairs(const MoeArgs& a, SortLds& s, const i
     s.first[tid] = first;
     for (int i = 0; i < mine; ++i) {
       s.item_expert[at + i] = (short)tid;
-      s.item_first[at + i] = (short)(first + i * 8);
-      s.item_count[at + i] = (short)min(8, n - i * 8);
+      s.item_first[at + i] = (short)(first + i * PER);
+      s.item_count[at + i] = (short)min(PER, n - i * PER);
     }
   }
   if (tid == NT - 1) s.items = upto & 0xffff;
@@ -422,12 +423,12 @@ __device__ __forceinline__ float pair_weight(const MoeArgs& a, const float* pick
 
 // One (item, part of I) after another of a wave's share, RT tiles of 16 rows of W2 from row `n0` on beside each other.  The loads
 // of a step are issued N - 1 steps before its products, across items too (named stages in turn: copying one into another
-// would wait for its loads).  HL: h lies in LDS, and the loads are the weights alone.
-template <class W, int RT, int N, bool HL>
+// would wait for its loads).  HL: h lies in LDS, and the loads are the weights alone.  PER: pairs of an item.
+template <class W, int RT, int N, bool HL, int PER>
 struct DownWave {
   struct Stage {
     Raw<W> w[RT];
-    RawValues h;                                     // (HL: read when it is used)
+    RawValues h[PER / 8];                            // (HL: read when it is used)
     const __bf16* row;
     float v;
     int kb, unit;                                    // unit: -1 - unit in its last step
@@ -470,8 +471,9 @@ struct DownWave {
     w = (const W*)a.w2 + ex * a.w2_e;
     // (RT tiles of 16 rows from a multiple of RT tiles lie in one block of 128)
     if constexpr (sizeof(W) == 1) sc = a.s2 + ((int64_t)ex * ((a.H + GROUP - 1) / GROUP) + n0 / GROUP) * KB;
-    const int pair = s.pair[first + min(r & 7, count - 1)];
-    if constexpr (HL) h = h_lds + (pair + (r < 8 ? 0 : a.T * a.k)) * (a.I + 8);
+    const int pair = s.pair[first + min(r & (PER - 1), count - 1)];
+    if constexpr (PER == 16) h = (const __bf16*)a.h_hi + (int64_t)pair * a.I;
+    else if constexpr (HL) h = h_lds + (pair + (r < 8 ? 0 : a.T * a.k)) * (a.I + 8);
     else h = (const __bf16*)(r < 8 ? a.h_hi : a.h_lo) + (int64_t)pair * a.I;
     kb = KB * part / parts;
     to = KB * (part + 1) / parts;
@@ -480,7 +482,8 @@ struct DownWave {
 #pragma unroll
     for (int t = 0; t < RT; ++t) q.w[t] = load_w<W>(w + w_row[t], kb * GROUP, g, a.I);
     if constexpr (HL) q.row = h;
-    else q.h = load_x<W>(h, kb * GROUP, g, a.I);
+    else q.h[0] = load_x<W>(h, kb * GROUP, g, a.I);
+    if constexpr (PER == 16) q.h[1] = load_x<W>(h + ((const __bf16*)a.h_lo - (const __bf16*)a.h_hi), kb * GROUP, g, a.I);
     if constexpr (sizeof(W) == 1) q.v = sc[kb];
     q.kb = kb;
     q.unit = unit;
@@ -490,18 +493,22 @@ struct DownWave {
       open();
     }
   }
-  // done(unit's item, part, sums of tile t: lane (r, g) has rows 4 g .. 4 g + 3 of the item's pair r, r < 8)
+  // done(unit's item, part, sums of tile t: lane (r, g) has rows 4 g .. 4 g + 3 of the item's pair r, r < PER)
   template <class F>
   __device__ __forceinline__ void multiply(Stage& q, F&& done) {
     if (q.kb >= full)
 #pragma unroll
       for (int t = 0; t < RT; ++t) clear_tail<W>(q.w[t], q.kb * GROUP, g, a.I);
-    if constexpr (HL) q.h = load_x<W>(q.row, q.kb * GROUP, g, a.I);
+    if constexpr (HL) q.h[0] = load_x<W>(q.row, q.kb * GROUP, g, a.I);
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       f32x4 d = sizeof(W) == 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[t];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d = Bf16Ops::mma(operand<Bf16Ops, W>(q.w[t], i), __builtin_bit_cast(bf16x8, q.h.v[i]), d);
+      for (int i = 0; i < 4; ++i) {
+        const bf16x8 f = operand<Bf16Ops, W>(q.w[t], i);
+#pragma unroll
+        for (int c = 0; c < PER / 8; ++c) d = Bf16Ops::mma(f, __builtin_bit_cast(bf16x8, q.h[c].v[i]), d);
+      }
       if constexpr (sizeof(W) == 1) add_scaled(acc[t], d, q.v);
       else acc[t] = d;
     }
@@ -510,7 +517,7 @@ struct DownWave {
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(acc[t][i]), 0x128, 0xf, 0xf, false));   // row_ror:8
+        for (int i = 0; i < 4 && PER == 8; ++i) acc[t][i] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(acc[t][i]), 0x128, 0xf, 0xf, false));   // row_ror:8
         done(which, unit - which * parts, t, acc[t]);
         acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
@@ -554,10 +561,10 @@ __device__ void down_few_kernel(const MoeArgs& a, float* partial) {
 #pragma unroll
   for (int i = 0; i < H_CHUNKS; ++i) hv[i] = ((const u32x4_a*)a.h_hi)[min(tid + i * NT, chunks - 1)];
   if (tid < pairs) picked[tid] = my_value;
-  sort_pairs<NT>(a, s, expert, [&](int pair, int at) { spot[pair] = at; });
+  sort_pairs<NT, 8>(a, s, expert, [&](int pair, int at) { spot[pair] = at; });
   const int parts = max(1, min(DOWN_WAVES / s.items, (a.I + GROUP - 1) / GROUP));
   __bf16* h_lds = (__bf16*)(partial + pairs * parts * 16);
-  DownWave<W, 1, 4, true> d(a, s, h_lds, blockIdx.x * 16, parts, wave, DOWN_WAVES);
+  DownWave<W, 1, 4, true, 8> d(a, s, h_lds, blockIdx.x * 16, parts, wave, DOWN_WAVES);
 #pragma unroll
   for (int i = 0; i < H_CHUNKS; ++i) {
     const int c = tid + i * NT, row = c / per_row;
@@ -591,7 +598,7 @@ __device__ void down_few_kernel(const MoeArgs& a, float* partial) {
 // y[part][pair][H] in 32 bits; combine_kernel adds them up.  Four tiles beside each other use a load of h four times: with one
 // (and all items in one block, no memory between) the loads' addresses took longer than the weights: 64 tokens, 8 of 128 experts
 // of 1024 x 4096 155 us, so 111 and 5 for the sum; 11 tokens, 2 of 8 of 4096 x 2048 in bf16 50, so 32 and 5.
-template <class W>
+template <class W, int PER>
 __device__ void down_many_kernel(const MoeArgs& a) {
   __shared__ SortLds s;
   constexpr int NT = DOWN_MANY_WAVES * 64;
@@ -599,12 +606,12 @@ __device__ void down_many_kernel(const MoeArgs& a) {
   int expert[MOE_T * MOE_K / NT];
 #pragma unroll
   for (int i = 0; i < MOE_T * MOE_K / NT; ++i) expert[i] = tid + i * NT < pairs ? a.ids[tid + i * NT] : 0;
-  sort_pairs<NT>(a, s, expert, [](int, int) {});
+  sort_pairs<NT, PER>(a, s, expert, [](int, int) {});
   const int waves = gridDim.y * DOWN_MANY_WAVES;
   const int parts = max(1, min(waves / s.items, a.max_parts));
   if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *a.parts = parts;
   const int n0 = blockIdx.x * DOWN_MANY_COLS;
-  DownWave<W, DOWN_MANY_COLS / 16, 2, false> d(a, s, nullptr, n0, parts, wave * gridDim.y + blockIdx.y, waves);
+  DownWave<W, DOWN_MANY_COLS / 16, 2, false, PER> d(a, s, nullptr, n0, parts, wave * gridDim.y + blockIdx.y, waves);
   d.run([&](int which, int part, int t, const f32x4& sum) {
     if (d.r < s.item_count[which] && n0 + t * 16 < a.H)
       *(f32x4*)(a.y + ((int64_t)part * pairs + s.pair[s.item_first[which] + d.r]) * a.H + n0 + t * 16 + d.g * 4) = sum;
