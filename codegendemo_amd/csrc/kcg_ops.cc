@@ -44,14 +44,15 @@ const Tile kTileTable[] = {
     {"32x32_2x1x4", 32, 32, 4, 512, {1.6f, .39f, 0.f}, {1.9f, .64f, 0.f}},        // 37 x 4096 x 4096: 7.4 us (64 x 64: 12.4)
     {"64x32_4x1x2", 64, 32, 2, 512, {1.2f, .36f, 0.f}, {1.4f, .62f, 0.f}},        // 37 x 8192 x 4096: 9.5 (32 x 32: 12.8, 64 x 64 by two: 10.8)
     {"64x64_2x2x1", 64, 64, 1, 256, {.4f, .305f, .52f}, {1.2f, .52f, .74f}},      // 512 x 4096 x 1024: 7.2 (by two: 10.8)
-    {"64x64_2x2x2", 64, 64, 2, 512, {1.9f, .43f, 0.f}, {2.2f, .76f, 0.f}},        // 256 x 4096 x 4096: 11.3 (by one: 12.8)
+    {"64x64_2x2x2", 64, 64, 2, 512, {1.9f, .47f, 0.f}, {2.2f, .76f, 0.f}},        // 256 x 4096 x 4096: 11.3 (by one: 12.8)
     {"64x128_2x2x1", 64, 128, 1, 256, {.8f, .6f, .67f}, {1.6f, .74f, 1.07f}},     // 4096 x 1536 x 1000, float32: 22.4 (64 x 64: 28.1, 128 x 128: 25.0)
     {"128x128_2x2x1", 128, 128, 1, 256, {1.6f, .655f, 1.1f}, {4.6f, 1.08f, 1.75f}},  // 2048 x 4096 x 4096: 39.8 (8 waves: 45.7)
-    // for 16-bit results only: the next is no faster than 64 x 128 with float32 ones, the last has no registers for them
+    // for 16-bit results only: the next two are no faster than 64 x 64 and 64 x 128 with float32 ones, the last has no registers for them
+    {"128x64_4x2x1", 128, 64, 1, 512, {.6f, .5f, 0.f}, {}},                       // 128 x 16384 x 4096: 23.0 (64 x 64: 27.0)
     {"128x128_4x2x1", 128, 128, 1, 512, {2.f, .575f, 0.f}, {}},                   // 1024 x 4096 x 4096: 23.5 (4 waves: 28.0)
     {"256x256_4x2x1", 256, 256, 1, 512, {7.f, 1.55f, 0.f}, {}},                   // 4096^3: 61.5 (128 x 128: 73.8)
 };
-constexpr int kTiles = sizeof(kTileTable) / sizeof(kTileTable[0]), kTilesF32 = kTiles - 2;
+constexpr int kTiles = sizeof(kTileTable) / sizeof(kTileTable[0]), kTilesF32 = kTiles - 3;
 constexpr double kLaunch = 2.3;
 
 double tile_estimate(const Tile& v, const Cost& c, int64_t m, int64_t n, int64_t groups) {

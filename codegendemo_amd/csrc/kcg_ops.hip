@@ -41,8 +41,8 @@ SWIGLU(float, f32)
 MATMULS(__bf16, bf16)
 MATMULS(_Float16, f16)
 MATMULS(float, f32)
-TILE(__bf16, bf16, 128, 128, 4, 2, 4, 1, 2) TILE(__bf16, bf16, 256, 256, 4, 2, 2, 1, 2)
-TILE(_Float16, f16, 128, 128, 4, 2, 4, 1, 2) TILE(_Float16, f16, 256, 256, 4, 2, 2, 1, 2)
+TILE(__bf16, bf16, 128, 64, 4, 2, 4, 1, 2) TILE(__bf16, bf16, 128, 128, 4, 2, 4, 1, 2) TILE(__bf16, bf16, 256, 256, 4, 2, 2, 1, 2)
+TILE(_Float16, f16, 128, 64, 4, 2, 4, 1, 2) TILE(_Float16, f16, 128, 128, 4, 2, 4, 1, 2) TILE(_Float16, f16, 256, 256, 4, 2, 2, 1, 2)
 
 #define MOE(OPS, W, X, NAME)                                                                                        \
   extern "C" __global__ void __launch_bounds__(UP_WAVES * 64, 4) kcg_moe_up_##NAME(MoeArgs a) { up_kernel<OPS, W, X>(a); } \

@@ -150,7 +150,7 @@ MATMULS = [(1, 1, 1, F32), (1, 16, 128, BF16), (2, 5, 15, F32), (3, 100, 127, F1
 # sizes that between them run every kernel (tests/test_ops_cpu.py checks that), with whole and partial groups of K, fewer groups
 # than a tile's waves split into, and counts that the split does not divide
 KERNEL_SIZES = [(1, 200, 700), (16, 8000, 300), (20, 100, 500), (30, 7300, 500), (24, 300, 2900), (64, 500, 1301), (37, 8100, 1100), (60, 8192, 129), (200, 300, 100),
-                (500, 4000, 260), (250, 4000, 4230), (300, 3000, 2050), (1000, 4000, 1290), (1000, 4000, 3500), (2000, 4000, 700), (4000, 4050, 1290), (4096, 4096, 3000)]
+                (500, 4000, 260), (250, 4000, 4230), (300, 3000, 2050), (8900, 70, 1285), (1000, 4000, 1290), (1000, 4000, 3500), (2000, 4000, 700), (4000, 4050, 1290), (4096, 4096, 3000)]
 
 
 @pytest.mark.parametrize("m,n,k", KERNEL_SIZES)

@@ -152,7 +152,7 @@ def test_the_tested_products_reach_every_kernel():
     reached = {_native_ops.matmul_fp8_kernel(m, n, k, c) for m, n, k in KERNEL_SIZES for c in (BF16, F16, F32)}
     with open(os.path.join(ROOT, "codegendemo_amd", "csrc", "kcg_ops.hsaco"), "rb") as f:
         built = {m.decode() for m in re.findall(rb"kcg_mm8_[a-z]+_[a-z0-9]+_[0-9x_]+(?=\0)", f.read())}
-    assert len(built) == 3 * 10 + 4 and reached == built
+    assert len(built) == 3 * 10 + 6 and reached == built
     assert _native_ops.matmul_fp8_kernel(0, 5, 5, BF16) == ""
     assert all(_native_ops.matmul_fp8_kernel(m, n, k, BF16) for m, n, k, _ in MATMULS)
     with pytest.raises(_native.KcgError):
