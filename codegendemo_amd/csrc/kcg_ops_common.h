@@ -125,17 +125,27 @@ __device__ __forceinline__ u32x2 quantize_group(const float (&v)[8], float& scal
   return u32x2{(unsigned)lo, (unsigned)hi};
 }
 
-// g / (1 + exp(-g)) * up to 8 half steps of float32 while exp(-g) is in range, and g * 0 * up behind it (g < -87), in two
+// g / (1 + exp(-g)) * up to 8 half steps of float32, g not below SILU_FAR, in two
 // transcendental and nine other instructions; expf and a division take some thirty.  exp(-g) = 2^p (1 + lo ln 2), where lo is
 // what the rounding of p = -g log2(e) left out (times |g| otherwise, which is what expf reduces its argument against).
-// lo counts only where 2^p is neither 0 nor infinite; the maximum keeps the factor positive (and not NaN) elsewhere, so that
-// an infinite 2^p gives 0 and g = infinity gives infinity.  NaN stays NaN through p.
+// The maximum keeps the factor positive, and not NaN where p is infinite: g = infinity gives infinity.  NaN stays NaN through p.
+constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596299e-8f, LN2 = 0.693147182f;
 __device__ __forceinline__ float silu_times(float g, float up) {
-  constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596299e-8f, LN2 = 0.693147182f;
   const float p = g * -LOG2E;
   const float lo = fmaf(g, -LOG2E_REST, fmaf(g, -LOG2E, -p));
   const float den = fmaf(__builtin_amdgcn_exp2f(p), fmaxf(fmaf(lo, LN2, 1.f), .5f), 1.f);
   return g * __builtin_amdgcn_rcpf(den) * up;
+}
+// The same below SILU_FAR, where 1 + exp(-g) is exp(-g): its reciprocal leaves the normal numbers at g = -87.3, while times a large
+// `up` the product does not.  So exp(g) is made 2^96 times too large (96 - p is exact: p lies in [115, 2^24) or is so large that
+// the power is 0) and the product is put right at the end.  To 6 half steps down to g = -154, 0 behind it, where |g exp(g) up| is
+// below 1e-26 for any `up`; g = -infinity gives NaN, as infinity times 0 does.
+constexpr float SILU_FAR = -80.f;
+__device__ __forceinline__ float silu_times_far(float g, float up) {
+  const float p = g * -LOG2E;
+  const float lo = fmaf(g, -LOG2E_REST, fmaf(g, -LOG2E, -p));
+  const float e = __builtin_amdgcn_exp2f(96.f - p) * fmaxf(fmaf(lo, -LN2, 1.f), .5f);
+  return g * e * up * 0x1p-96f;
 }
 
 // 8 bytes of a quantised row whose start is 16-byte aligned; bytes behind the row's end stay as they were

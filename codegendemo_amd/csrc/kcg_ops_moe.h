@@ -235,7 +235,7 @@ __device__ __forceinline__ void up_tiles(const MoeArgs& a, RouteLds& s, f32x4* r
   auto write = [&](int n, int row, float gate, float up) {
     const int t = s.token[n];
     const int64_t o = (int64_t)(t * a.k + s.rank[t]) * a.I + row;
-    const float h = silu_times(gate, up);
+    const float h = gate < SILU_FAR ? silu_times_far(gate, up) : silu_times(gate, up);
     const __bf16 hi = (__bf16)h;
     const float hf = (float)hi;
     ((__bf16*)a.h_hi)[o] = hi;

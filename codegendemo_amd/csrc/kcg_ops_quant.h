@@ -128,10 +128,19 @@ __device__ void swiglu_kernel(const SwigluArgs& a) {
   float g[8], u[8];
   load8(g, in, n);
   load8(u, in + a.cols, n);
+  float h[8];
+  unsigned far = 0;                               // (as unsigned integers, negative floats lie above the others, the smallest highest)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) g[i] = silu_times(g[i], u[i]);      // (behind the row: 0 times 0)
+  for (int i = 0; i < 8; ++i) {
+    h[i] = silu_times(g[i], u[i]);                // (behind the row: 0 times 0)
+    far = max(far, __float_as_uint(g[i]));
+  }
+  if (far > __float_as_uint(SILU_FAR)) {          // (hardly ever: one comparison for eight values)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = g[i] < SILU_FAR ? silu_times_far(g[i], u[i]) : h[i];
+  }
   float scale;
-  const u32x2 q = quantize_group(g, scale);
+  const u32x2 q = quantize_group(h, scale);
   if (n > 0) {
     store_q8(a.q + (int64_t)row * a.q_stride + c, q, n);
     if ((c & (GROUP - 1)) == 0) a.scale[(int64_t)row * a.scale_stride_t + (int64_t)(c / GROUP) * a.scale_stride_g] = scale;
