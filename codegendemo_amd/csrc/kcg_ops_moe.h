@@ -50,8 +50,8 @@ struct RawValues {
   u32x4 v[4];
 };
 // The loads have no branches (behind one, the compiler could not count which loads are in flight, and would wait for all of
-// them): a place at or behind `n` (a multiple of 16) is read from the row's last values instead, and clear_tail() makes the
-// weights there zero.
+// them): a place at or behind `n` (a multiple of 16) is read from the row's last values instead, and clear_tail() makes it zero,
+// in weights and values both: either may hold an infinity there, and 0 times that is NaN.
 template <class W>
 __device__ __forceinline__ Raw<W> load_w(const W* row, int k, int g, int n) {
   Raw<W> q;
@@ -73,6 +73,12 @@ __device__ __forceinline__ void clear_tail(Raw<W>& q, int k, int g, int n) {
 #pragma unroll
   for (int i = 0; i < C; ++i)
     if (k + place<W>(g, i * (4 / C)) >= n) q.v[i] = u32x4{0u, 0u, 0u, 0u};
+}
+template <class W>
+__device__ __forceinline__ void clear_tail(RawValues& q, int k, int g, int n) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (k + place<W>(g, i) >= n) q.v[i] = u32x4{0u, 0u, 0u, 0u};
 }
 template <class Ops, class W>
 __device__ __forceinline__ typename Ops::vec operand(const Raw<W>& q, int i) {
@@ -248,6 +254,8 @@ __device__ __forceinline__ void up_tiles(const MoeArgs& a, RouteLds& s, f32x4* r
     if (kb >= full) {
       clear_tail<W>(st.g, kb * GROUP, g, a.H);
       clear_tail<W>(st.u, kb * GROUP, g, a.H);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) clear_tail<W>(st.x[c], kb * GROUP, g, a.H);
     }
     f32x4 dg[CT], du[CT];
 #pragma unroll
@@ -496,10 +504,13 @@ struct DownWave {
   // done(unit's item, part, sums of tile t: lane (r, g) has rows 4 g .. 4 g + 3 of the item's pair r, r < PER)
   template <class F>
   __device__ __forceinline__ void multiply(Stage& q, F&& done) {
-    if (q.kb >= full)
+    if constexpr (HL) q.h[0] = load_x<W>(q.row, q.kb * GROUP, g, a.I);
+    if (q.kb >= full) {
 #pragma unroll
       for (int t = 0; t < RT; ++t) clear_tail<W>(q.w[t], q.kb * GROUP, g, a.I);
-    if constexpr (HL) q.h[0] = load_x<W>(q.row, q.kb * GROUP, g, a.I);
+#pragma unroll
+      for (int c = 0; c < PER / 8; ++c) clear_tail<W>(q.h[c], q.kb * GROUP, g, a.I);
+    }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       f32x4 d = sizeof(W) == 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[t];

@@ -8,6 +8,7 @@ from tests import ops_reference as R
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+E4M3 = torch.float8_e4m3fn
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 # ---- gates far below zero: exp(gate) is small, exp(gate) * up need not be ----------------------------------------------------
@@ -51,3 +52,51 @@ def test_moe_of_far_gates(t, gate):
     out = moe_layer(x, torch.zeros(t, 1, device=DEV), 1, w13, w2)[0]
     want = torch.tensor(gate, dtype=torch.float64).sigmoid().item() * gate * 2.0 ** 126
     assert bool(((out.double() - want).abs() <= abs(want) * (R.half_step(BF16) + R.SWIGLU_REL + 2.0 ** -18)).all())
+
+
+# ---- infinities where a row's last group of 128 is partial -------------------------------------------------------------------
+
+def constant_experts(weights, h, i, fill13, fill2):
+    """One expert of equal weights, e4m3 ones with scales of 1."""
+    w13, w2 = torch.full((1, 2 * i, h), fill13, device=DEV).to(weights), torch.full((1, h, i), fill2, device=DEV).to(weights)
+    if weights is BF16:
+        return w13, w2, None, None
+    return w13, w2, torch.ones(1, R.groups(2 * i), R.groups(h), device=DEV), torch.ones(1, R.groups(h), R.groups(i), device=DEV)
+
+
+EXPERT_TYPES = [(E4M3, BF16), (E4M3, F16), (BF16, BF16)]
+
+
+@pytest.mark.parametrize("weights,dtype", EXPERT_TYPES)
+@pytest.mark.parametrize("t", [1, 4, 8, 12, 24, 40])
+@pytest.mark.parametrize("h", [16, 144, 240])
+def test_moe_of_an_infinity_in_a_ragged_row(t, h, weights, dtype):
+    """Positive weights and an infinite value of one token: its sums are infinite, not NaN, wherever in its row the value stands."""
+    w13, w2, s13, s2 = constant_experts(weights, h, 128, 0.5, 0.25)
+    logits = torch.zeros(t, 1, device=DEV)
+    x = torch.ones(t, h, device=DEV).to(dtype)
+    clean = moe_layer(x, logits, 1, w13, w2, s13, s2)[0]
+    for at in (0, h - 9, h - 8, h - 1):
+        y = x.clone()
+        y[t // 2, at] = float("inf")
+        out = moe_layer(y, logits, 1, w13, w2, s13, s2)[0]
+        assert bool((out[t // 2] == float("inf")).all()), at
+        keep = torch.arange(t) != t // 2
+        assert torch.equal(out[keep], clean[keep])
+
+
+@pytest.mark.parametrize("weights,dtype", EXPERT_TYPES)
+@pytest.mark.parametrize("t", [1, 4, 8, 24])
+@pytest.mark.parametrize("i", [16, 144, 240])
+def test_moe_of_an_infinite_activation_in_a_ragged_row(t, i, weights, dtype):
+    """One of the activations between the products passes float32's range, the others are 0: the second product is infinite, not NaN."""
+    h = 128
+    for at in (0, i - 9, i - 8, i - 1):
+        w13, w2, s13, s2 = constant_experts(weights, h, i, 0.0, 0.25)
+        if weights is BF16:
+            w13[0, at] = w13[0, i + at] = 1e30
+        else:
+            w13[0, at] = w13[0, i + at] = 1.0
+            s13.fill_(1e30)
+        out = moe_layer(torch.ones(t, h, device=DEV).to(dtype), torch.zeros(t, 1, device=DEV), 1, w13, w2, s13, s2)[0]
+        assert bool((out == float("inf")).all()), at
