@@ -137,7 +137,8 @@ int fail(int code, const std::string& msg) {
   X(hipEventDestroy)          \
   X(hipStreamSynchronize)     \
   X(hipGetDeviceProperties)   \
-  X(hipGetErrorString)
+  X(hipGetErrorString)        \
+  X(hipGetLastError)
 
 #define KCG_RTC_FUNCS(X)      \
   X(hiprtcCreateProgram)      \
@@ -253,9 +254,11 @@ const RtcLib& rtc_lib() {
 
 #define HIPF(name) (hip_api().p_##name)
 
-// Same text shape as the reference loader's errors (loaderCCode/hip.c:8-21).
+// Same text shape as the reference loader's errors (loaderCCode/hip.c:8-21).  The failure is reported here, so the runtime's
+// record of it is cleared: left standing, it would be taken for a failure of the host program's next launch.
 int hip_fail(hipError_t e, const char* what) {
   char buf[1024];
+  if (hip_api().ok) (void)HIPF(hipGetLastError)();
   const char* txt = hip_api().ok ? HIPF(hipGetErrorString)(e) : "?";
   snprintf(buf, sizeof(buf), "KCG Error[HIP]:  Code: %d, Messsage: %s (%s)", (int)e, txt, what);
   g_err = buf;

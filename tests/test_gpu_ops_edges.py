@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from codegendemo_amd import _native, _native_ops
 from codegendemo_amd.kcg.Operators.moe import moe_layer
 from codegendemo_amd.kcg.Operators.quant import swiglu_quant
 from tests import ops_reference as R
@@ -100,3 +101,14 @@ def test_moe_of_an_infinite_activation_in_a_ragged_row(t, i, weights, dtype):
             s13.fill_(1e30)
         out = moe_layer(torch.ones(t, h, device=DEV).to(dtype), torch.zeros(t, 1, device=DEV), 1, w13, w2, s13, s2)[0]
         assert bool((out == float("inf")).all()), at
+
+
+# ---- a failed call is over when it has been reported -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("refused", [_native_ops.load, _native.device_info])
+def test_a_reported_failure_is_not_reported_again(refused):
+    """A device number that does not exist fails on the host; the program's next launch has nothing to do with it."""
+    with pytest.raises(_native.KcgError) as e:
+        refused(99)
+    assert e.value.status == _native.ERR_HIP
+    assert (torch.ones(4, device=DEV) * 3).sum().item() == 12
