@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ops/empty_strided.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -44,6 +45,16 @@ const at::Tensor& tensor(const char* name, PyObject* o) {
   return THPVariable_Unpack(o);
 }
 
+// The operators have no backward pass.  Results cut off from an argument that wants a gradient would train wrongly without a word,
+// so such a call is refused, as torch refuses its own functions with an out argument.
+void no_gradient(PyObject* const* a, Py_ssize_t n) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (Py_ssize_t i = 0; i < n; ++i)
+    TORCH_CHECK(!THPVariable_Check(a[i]) || !THPVariable_Unpack(a[i]).requires_grad(),
+                "the operators of the 8-bit path have no gradient, and a tensor of the call requires one (shape ", THPVariable_Unpack(a[i]).sizes(),
+                "): call under torch.no_grad(), or pass its detach()");
+}
+
 void on_gpu(const char* name, const at::Tensor& t) {
   TORCH_CHECK_TYPE(t.is_cuda(), name, " must be on a GPU, got ", t.device().str(), ": the operators have no CPU path");
 }
@@ -66,6 +77,7 @@ int64_t matrix(const char* name, const at::Tensor& t, int64_t rows, int64_t cols
 struct Matrix {
   int64_t address = 0, row = 0, col = 0;
   PyObject* object = nullptr;                // a new reference, or null
+  bool theirs = false;                       // an output that the caller passed in
   Matrix() = default;
   Matrix(const Matrix&) = delete;
   ~Matrix() { Py_XDECREF(object); }
@@ -81,6 +93,13 @@ struct Matrix {
     col = 1;
     object = THPVariable_Wrap(std::move(t));
     if (!object) throw python_error();
+  }
+  // a tensor of the caller's has been written: what autograd has saved of it counts as changed (a tensor of inference mode keeps
+  // no such count)
+  void written() const {
+    if (!theirs) return;
+    const at::Tensor& t = THPVariable_Unpack(object);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   }
   void given(const char* name, PyObject* o, int64_t rows, int64_t cols, ScalarType type, at::Device device) {
     const at::Tensor& t = tensor(name, o);
@@ -102,12 +121,14 @@ struct Matrix {
       made(rows, cols, ld, type, device);
     else
       given(name, o, rows, cols, type, device);
+    theirs = o != Py_None;
   }
   void output_scales(PyObject* o, int64_t rows, int64_t cols, at::Device device) {
     if (o == Py_None)
       made(rows, cols, cols, ScalarType::Float, device);
     else
       given_any_strides("scale", o, rows, cols, device);
+    theirs = o != Py_None;
   }
 };
 
@@ -166,6 +187,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* rmsnorm_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!count("rmsnorm_quant", n, 9)) return nullptr;
+  no_gradient(a, n);
   const at::Tensor& x = tensor("x", a[0]);
   on_gpu("x", x);
   TORCH_CHECK_VALUE(x.dim() == 2, "x must be a matrix, got shape ", x.sizes());
@@ -204,7 +226,10 @@ PyObject* rmsnorm_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.q = q.address, p.q_stride = q.row;
   p.scale = scale.address, p.scale_stride_row = scale.row, p.scale_stride_group = scale.col;
   p.y = y.address, p.y_stride = y.row;
-  if (p.rows && p.cols && !run(norm_entry, p, device.index())) return nullptr;
+  if (p.rows && p.cols) {
+    if (!run(norm_entry, p, device.index())) return nullptr;
+    for (const Matrix* m : {&residual_out, &q, &scale, &y}) m->written();
+  }
   PyObject* r = PyTuple_New(4);
   if (!r) return nullptr;
   PyTuple_SET_ITEM(r, 0, q.release());
@@ -219,6 +244,7 @@ PyObject* rmsnorm_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* swiglu_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!count("swiglu_quant", n, 3)) return nullptr;
+  no_gradient(a, n);
   const at::Tensor& gate_up = tensor("gate_up", a[0]);
   on_gpu("gate_up", gate_up);
   TORCH_CHECK_VALUE(gate_up.dim() == 2 && gate_up.size(1) % 2 == 0, "gate_up must be a matrix with an even number of columns, got shape ", gate_up.sizes());
@@ -236,7 +262,10 @@ PyObject* swiglu_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
   scale.output_scales(a[2], p.rows, groups(p.cols), device);
   p.q = q.address, p.q_stride = q.row;
   p.scale = scale.address, p.scale_stride_row = scale.row, p.scale_stride_group = scale.col;
-  if (p.rows && p.cols && !run(swiglu_entry, p, device.index())) return nullptr;
+  if (p.rows && p.cols) {
+    if (!run(swiglu_entry, p, device.index())) return nullptr;
+    for (const Matrix* m : {&q, &scale}) m->written();
+  }
   PyObject* r = PyTuple_New(2);
   if (!r) return nullptr;
   PyTuple_SET_ITEM(r, 0, q.release());
@@ -249,6 +278,7 @@ PyObject* swiglu_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* matmul_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!count("matmul_fp8", n, 6)) return nullptr;
+  no_gradient(a, n);
   const at::Tensor &ta = tensor("a", a[0]), &tb = tensor("b", a[2]);
   on_gpu("a", ta);
   TORCH_CHECK_VALUE(ta.dim() == 2 && tb.dim() == 2, "a and b must be matrices, got shapes ", ta.sizes(), " and ", tb.sizes());
@@ -277,7 +307,10 @@ PyObject* matmul_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.a_scale = sa.address, p.a_scale_stride_row = sa.row, p.a_scale_stride_group = sa.col;
   p.b_scale = sb.address, p.b_scale_stride_row = sb.row, p.b_scale_stride_group = sb.col;
   p.c = out.address, p.c_stride = out.row;
-  if (p.m && p.n && !run(matmul_entry, p, device.index())) return nullptr;
+  if (p.m && p.n) {
+    if (!run(matmul_entry, p, device.index())) return nullptr;
+    out.written();
+  }
   return out.release();
   END_HANDLE_TH_ERRORS
 }
@@ -303,6 +336,7 @@ int64_t block_scales(const char* name, PyObject* o, const at::Tensor& w, at::Dev
 PyObject* moe_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!count("moe_layer", n, 9)) return nullptr;
+  no_gradient(a, n);
   const at::Tensor &x = tensor("x", a[0]), &logits = tensor("logits", a[1]), &w13 = tensor("w13", a[3]), &w2 = tensor("w2", a[4]);
   on_gpu("x", x);
   TORCH_CHECK_VALUE(x.dim() == 2 && logits.dim() == 2 && w13.dim() == 3, "x and logits must be matrices, w13 and w2 [experts, rows, columns]");
@@ -353,6 +387,7 @@ PyObject* moe_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor workspace = at::empty_strided({p.workspace_bytes}, {1}, at::TensorOptions().dtype(ScalarType::Byte).device(device));
     p.workspace = address(workspace);
     if (!run(moe_entry, p, device.index())) return nullptr;
+    out.written();
   }
   PyObject* r = PyTuple_New(3);
   if (!r) return nullptr;

@@ -165,3 +165,19 @@ def test_operator_check_command_refuses(argv, capsys):
     with pytest.raises(SystemExit) as e:
         single.main(argv)
     assert e.value.code == 2 and "error" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("call", [
+    lambda x: rmsnorm_quant(torch.zeros(2, 128), x[0]), lambda x: rmsnorm_quant(torch.zeros(2, 128), torch.zeros(128), residual=x), lambda x: swiglu_quant(x),
+    lambda x: matmul_fp8(torch.zeros(2, 128), x, torch.zeros(2, 128), torch.zeros(1, 1)), lambda x: matmul_fp8(x.detach(), x.detach(), x.detach(), x.detach(), out=x),
+    lambda x: moe_layer(torch.zeros(2, 16), x, 1, torch.zeros(128, 32, 16), torch.zeros(128, 16, 16)),
+    lambda x: moe_layer(torch.zeros(2, 16), torch.zeros(2, 1), 1, x[None], torch.zeros(1, 16, 16))])
+def test_a_tensor_that_requires_a_gradient_is_refused(call):
+    """... before anything else; without gradients the same call gets as far as finding no GPU."""
+    x = torch.zeros(2, 128, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient.*no_grad"):
+        call(x)
+    with torch.no_grad(), pytest.raises(TypeError, match="GPU"):
+        call(x)
+    with torch.inference_mode(), pytest.raises(TypeError, match="GPU"):
+        call(x)
