@@ -159,3 +159,58 @@ def test_parameters_without_a_gradient_are_served():
     with torch.no_grad():
         assert not rmsnorm_quant(x, w, want_y=True)[2].requires_grad
     assert not rmsnorm_quant(x, w.requires_grad_(False), want_y=True)[2].requires_grad
+
+
+# ---- products that cancel, and channels far above the others -----------------------------------------------------------------
+
+# a size for each way the product is cut: few rows (one and two row tiles), K shared by waves, tiles of 64 to 256
+CANCEL_SIZES = [(1, 300, 520), (20, 100, 500), (40, 300, 1301), (64, 1000, 520), (200, 300, 700), (500, 4000, 260), (1000, 4000, 1290), (4000, 4050, 1290)]
+
+
+def check_stated_bound(c, a, sa, b, sb):
+    """float32: 128 terms of a group and the groups' sums at 2 roundings each, the scales' two products.  16 bits: besides these 2^-10 of
+    the sum of magnitudes, as documented, and the result's own rounding."""
+    wa, wb = R.widen(a, sa, False), R.widen(b, sb, True)
+    want, size = wa @ wb.t().contiguous(), wa.abs() @ wb.abs().t().contiguous()
+    allowed = size * (2 * (128 + R.groups(a.shape[1])) + 4) * R.U
+    if c.dtype is not F32:
+        allowed += size * 2.0 ** -10
+    allowed = allowed * (1 + R.half_step(c.dtype)) + want.abs() * R.half_step(c.dtype) + R.smallest(c.dtype)
+    off = (c.double() - want).abs()
+    assert bool((off <= allowed).all()), f"off by up to {(off / allowed).max().item()} of what is allowed"
+    return want
+
+
+@pytest.mark.parametrize("m,n,k", CANCEL_SIZES)
+@pytest.mark.parametrize("out", [BF16, F16, F32])
+def test_matmul_of_products_that_cancel(m, n, k, out):
+    """448 * 448 - 448 * 448 and six products of 14 in every 8: whole numbers below 2^24 times the scale, which float32 sums hold
+    exactly (one row and one block of scales each, so that the groups' factors do not differ); 16-bit results are held to their bound."""
+    a = torch.tensor([448.0, 448.0] + [3.5] * 6, device=DEV).repeat(m, R.groups(k) * 16)[:, :k].to(E4M3).contiguous()
+    b = torch.tensor([448.0, -448.0] + [4.0] * 6, device=DEV).repeat(n, R.groups(k) * 16)[:, :k].to(E4M3).contiguous()
+    pad = -k % 16
+    a, b = (torch.nn.functional.pad(v.view(torch.uint8), (0, pad), value=0x7f).view(E4M3)[:, :k] for v in (a, b))
+    sa, sb = torch.full((m, R.groups(k)), 2.0 ** -8, device=DEV), torch.full((R.groups(n), R.groups(k)), 0.5, device=DEV)
+    c = matmul_fp8(a, sa, b, sb, out_dtype=out)
+    want = check_stated_bound(c, a, sa, b, sb)
+    if out is F32:
+        assert torch.equal(c.double(), want)
+
+
+@pytest.mark.parametrize("m,n,k", CANCEL_SIZES)
+@pytest.mark.parametrize("out", [BF16, F16, F32])
+def test_matmul_of_channels_far_above_the_others(m, n, k, out):
+    """A few channels of a hundred times the others' size, as activations have them: their groups' other values stand on a coarse scale."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(m + n + k)
+
+    def quantised(rows, block):
+        v = torch.zeros(-(-rows // block) * block, R.groups(k) * 128, device=DEV)
+        v[:rows, :k] = torch.randn(rows, k, device=DEV, generator=g) * (1 + 100 * (torch.rand(k, device=DEV, generator=g) < 0.02))
+        v = v.view(-1, block, R.groups(k), 128)
+        s = v.abs().amax((1, 3)).clamp_min(1e-10) / 448
+        return (v / s[:, None, :, None]).view(-1, R.groups(k) * 128).to(E4M3)[:rows, :k], s.contiguous()
+
+    (a, sa), (b, sb) = quantised(m, 1), quantised(n, 128)
+    sa *= 2.0 ** -5                                        # (two of the large channels may meet: their products stay below float16's largest)
+    check_stated_bound(matmul_fp8(a, sa, b, sb, out_dtype=out), a, sa, b, sb)
