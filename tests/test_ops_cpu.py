@@ -181,3 +181,38 @@ def test_a_tensor_that_requires_a_gradient_is_refused(call):
         call(x)
     with torch.inference_mode(), pytest.raises(TypeError, match="GPU"):
         call(x)
+
+
+def built_kernels(pattern):
+    with open(os.path.join(ROOT, "codegendemo_amd", "csrc", "kcg_ops.hsaco"), "rb") as f:
+        return {m.decode() for m in re.findall(rb"(?:%s)(?=\0)" % pattern, f.read())}
+
+
+def parameters(test):
+    """What a test is parametrised over: {names: values}."""
+    return {m.args[0]: m.args[1] for m in test.pytestmark if m.name == "parametrize"}
+
+
+def test_every_product_kernel_is_run():
+    """From the very lists that the GPU tests run over, types included."""
+    from tests import test_gpu_ops, test_gpu_ops_kernels
+    codes = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
+    run = set()
+    for test in (test_gpu_ops.test_matmul_kernels, test_gpu_ops_kernels.test_matmul_kernels_in_float16):
+        p = parameters(test)
+        run |= {_native_ops.matmul_fp8_kernel(m, n, k, codes[out]) for m, n, k in p["m,n,k"] for out in p["out"]}
+    built = built_kernels(rb"kcg_mm8_[a-z]+_[a-z0-9]+_[0-9x_]+")
+    assert built and run == built, sorted(built - run)
+
+
+def test_every_norm_kernel_is_run():
+    """A kernel's name says how many threads a row gets and how many vectors of 8 each holds (0: any number)."""
+    from tests import test_gpu_ops, test_gpu_ops_kernels
+    names = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+    built = built_kernels(rb"kcg_norm_[a-z0-9]+_[0-9]+_[0-9]+")
+    holds = sorted({(int(nt) * int(v) * 8 or 1 << 62, f"{nt}_{v}") for nt, v in (b.split("_")[3:] for b in built)})
+    run = set()
+    for test in (test_gpu_ops.test_norm, test_gpu_ops_kernels.test_norm_kernels):
+        for _, h, dtype in parameters(test)["t,h,dtype"]:
+            run.add(f"kcg_norm_{names[dtype]}_" + next(name for most, name in holds if h <= most))
+    assert len(built) == 21 and run == built, sorted(built - run)
