@@ -124,7 +124,6 @@ int fail(int code, const std::string& msg) {
 #define KCG_HIP_FUNCS(X)      \
   X(hipSetDevice)             \
   X(hipGetDevice)             \
-  X(hipGetDeviceCount)        \
   X(hipModuleLoadData)        \
   X(hipModuleGetFunction)     \
   X(hipModuleUnload)          \
@@ -432,9 +431,9 @@ const HostHip* host_hip() {
     fail(KCG_ERR_HIP, "KCG Error[HIP]: runtime unavailable:" + hip_api().error);
     return nullptr;
   }
-  static const HostHip h = {HIPF(hipGetDevice),       HIPF(hipSetDevice),         HIPF(hipGetDeviceCount),
-                            HIPF(hipModuleLoadData),  HIPF(hipModuleGetFunction), HIPF(hipModuleUnload),
-                            HIPF(hipModuleLaunchKernel), hip_api().p_hipFuncSetAttribute};
+  static const HostHip h = {HIPF(hipGetDevice),          HIPF(hipSetDevice),    HIPF(hipModuleLoadData),
+                            HIPF(hipModuleGetFunction),  HIPF(hipModuleUnload), HIPF(hipModuleLaunchKernel),
+                            hip_api().p_hipFuncSetAttribute};
   return &h;
 }
 

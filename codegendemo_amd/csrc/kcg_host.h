@@ -9,7 +9,6 @@ namespace kcg {
 struct HostHip {
   decltype(&::hipGetDevice) GetDevice;
   decltype(&::hipSetDevice) SetDevice;
-  decltype(&::hipGetDeviceCount) GetDeviceCount;
   decltype(&::hipModuleLoadData) ModuleLoadData;
   decltype(&::hipModuleGetFunction) ModuleGetFunction;
   decltype(&::hipModuleUnload) ModuleUnload;
