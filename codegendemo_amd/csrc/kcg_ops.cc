@@ -14,9 +14,13 @@
 #include "kcg_host.h"
 #include "kcg_ops_args.h"
 
-// the code object of kcg_ops.hip
+// the code object of kcg_ops.hip; empty in a library that was built where there is no hipcc
+#ifdef KCG_OPS_CODE
 __asm__(".section .rodata\n.balign 4096\n.global kcg_ops_code\nkcg_ops_code:\n.incbin \"" KCG_OPS_CODE "\"\n.byte 0\n.previous\n");
 extern "C" const char kcg_ops_code[];
+#else
+static const char kcg_ops_code[] = "";
+#endif
 
 namespace {
 
@@ -217,6 +221,7 @@ int launch(const HostHip* hip, hipFunction_t fn, unsigned gx, unsigned gy, unsig
 template <class F>
 int on_device(int device, F f) {
   try {
+    if (!*kcg_ops_code) return host_fail(KCG_ERR_COMPILE, "the library was built without hipcc and has no kernels of the operators: build it again with hipcc");
     const HostHip* hip = host_hip();
     if (!hip) return KCG_ERR_HIP;
     OnDevice guard(hip, device);

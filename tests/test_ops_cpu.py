@@ -1,6 +1,8 @@
 """The operators of the 8-bit path where no GPU is needed: the ABI, every refusal that comes before a launch, empty calls."""
 import os
 import re
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -216,3 +218,22 @@ def test_every_norm_kernel_is_run():
         for _, h, dtype in parameters(test)["t,h,dtype"]:
             run.add(f"kcg_norm_{names[dtype]}_" + next(name for most, name in holds if h <= most))
     assert len(built) == 21 and run == built, sorted(built - run)
+
+
+def test_the_library_is_built_without_hipcc(tmp_path):
+    """The tuned products' host side needs a C++ compiler alone; the operators say what is missing, and refuse bad arguments as ever."""
+    out = tmp_path / "libkcg_gemm.so"
+    made = subprocess.run(["make", "-C", _native.CSRC_DIR, f"OUT={out}", f"HIPCC={tmp_path}/hipcc", str(out)], capture_output=True, text=True)
+    assert made.returncode == 0, made.stderr
+    assert "without the kernels of the operators" in made.stderr
+    code = f"""
+import ctypes
+L = ctypes.CDLL({str(out)!r})
+L.kcg_last_error.restype = L.kcg_version.restype = ctypes.c_char_p
+assert L.kcg_version()
+assert L.kcg_ops_load(0) == {_native.ERR_COMPILE}
+assert b"without hipcc" in L.kcg_last_error()
+assert L.kcg_matmul_fp8(None, 0, 0) == {_native.ERR_ARGUMENT}
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr
