@@ -261,7 +261,7 @@ bool scale_layout_ok(int64_t row, int64_t group, int64_t rows, int64_t ng) {
   if (!any_stride_ok(row) || !any_stride_ok(group)) return false;
   if (rows > 1 && row == 0) return false;
   if (ng > 1 && group == 0) return false;
-  if (rows > 1 && ng > 1) return row >= group * ng || group >= row * rows;
+  if (rows > 1 && ng > 1) return row > group * (ng - 1) || group > row * (rows - 1);
   return true;
 }
 

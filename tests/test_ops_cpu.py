@@ -237,3 +237,23 @@ assert L.kcg_matmul_fp8(None, 0, 0) == {_native.ERR_ARGUMENT}
 """
     run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert run.returncode == 0, run.stderr
+
+
+def accepted(name, change):
+    """The arguments pass every check: what fails then is finding a GPU."""
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are not a GPU's")
+    with pytest.raises(_native.KcgError) as e:
+        call(name, {**GOOD[name], **change})
+    assert e.value.status == _native.ERR_HIP, str(e.value)
+
+
+@pytest.mark.parametrize("name", ["kcg_rmsnorm_quant", "kcg_swiglu_quant"])
+def test_scales_that_lie_between_others_do_not_overlap(name):
+    """Three groups a row, every second of 5 neighbours: 0 2 4, 5 7 9, ...; transposed the same; one further apart or closer is refused."""
+    three = dict(cols=300, q_stride=304, **({"x_stride": 300, "residual_stride": 300, "residual_out_stride": 300, "y_stride": 300} if "norm" in name else {"gate_up_stride": 600}))
+    accepted(name, dict(three, scale_stride_row=5, scale_stride_group=2))
+    accepted(name, dict(three, scale_stride_row=2, scale_stride_group=7))
+    for row, group in ((4, 2), (2, 6)):
+        with pytest.raises(_native.KcgError, match="overlap"):
+            call(name, {**GOOD[name], **three, "scale_stride_row": row, "scale_stride_group": group})
