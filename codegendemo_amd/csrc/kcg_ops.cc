@@ -396,8 +396,8 @@ int kcg_moe_layer(const kcg_moe_layer_args* p, int device, uint64_t stream) {
       !aligned(p->w2_scale, 4))
     return bad("moe_layer: an address is not aligned to its elements");
   const int64_t wb = type_bytes(p->weight_dtype), per16 = 16 / wb;
-  if (!aligned(p->w13, 16) || !aligned(p->w2, 16) || !aligned(p->workspace, 16) || !aligned(p->w13_stride_expert, per16) ||
-      !aligned(p->w13_stride_row, per16) || !aligned(p->w2_stride_expert, per16) || !aligned(p->w2_stride_row, per16))
+  if (!aligned(p->w13, 16) || !aligned(p->w2, 16) || !aligned(p->workspace, 16) || !aligned(p->w13_stride_row, per16) ||
+      !aligned(p->w2_stride_row, per16) || (p->experts > 1 && (!aligned(p->w13_stride_expert, per16) || !aligned(p->w2_stride_expert, per16))))
     return bad("moe_layer: the workspace and the rows of w13 and w2 must start on 16 bytes");
   if (!stride_ok(p->x_stride, p->hidden, 1) || !stride_ok(p->out_stride, p->hidden, p->tokens) || !any_stride_ok(p->logits_stride) ||
       !any_stride_ok(p->w13_stride_expert) || !any_stride_ok(p->w13_stride_row) || !any_stride_ok(p->w2_stride_expert) ||

@@ -257,3 +257,11 @@ def test_scales_that_lie_between_others_do_not_overlap(name):
     for row, group in ((4, 2), (2, 6)):
         with pytest.raises(_native.KcgError, match="overlap"):
             call(name, {**GOOD[name], **three, "scale_stride_row": row, "scale_stride_group": group})
+
+
+def test_one_expert_has_no_stride_to_another():
+    """A view of a lone expert's weights may name any stride for it."""
+    accepted("kcg_moe_layer", dict(experts=1, topk=1, w13_stride_expert=1, w2_stride_expert=3))
+    for change in (dict(w13_stride_expert=1), dict(w2_stride_expert=3)):
+        with pytest.raises(_native.KcgError, match="16 bytes"):
+            call("kcg_moe_layer", {**GOOD["kcg_moe_layer"], **change})
