@@ -14,8 +14,8 @@
  *
  * Rows of 8-bit operands start on 16 bytes: base addresses and row strides are multiples of 16 (the row length is not
  * bound: what lies between its end and the next multiple of 16 is not written, and when read does not count, whatever it
- * holds).  Strides are in elements.  `device` is the device the memory and the stream belong to; the calling
- * thread's current device is the same before and after.
+ * holds).  Strides are in elements.  Outputs overlap neither inputs nor each other where nothing else is said.  `device` is the
+ * device the memory and the stream belong to; the calling thread's current device is the same before and after.
  *
  * The first call on a device loads the library's code object there, which must not happen inside a stream capture: call
  * kcg_ops_load (or the operator once) before.  Afterwards every call can be captured into a HIP graph.
@@ -84,8 +84,9 @@ int kcg_matmul_fp8_kernel(int64_t m, int64_t n, int64_t k, int64_t c_dtype, char
 /* A layer of routed experts for at most 64 tokens: the topk largest logits of a token (equal ones: the lower index) choose
  * its experts, p = softmax over them (renormalize) or over all experts,
  *   h_e = silu(W1_e x) * (W3_e x),   out = sum_e p_e W2_e h_e,
- * W1 the first `inter` rows of w13[e], W3 the others.  A logit of -infinity takes an expert out: if it is among the
- * topk all the same its weight is 0 and it adds nothing; a token with no other logits gets zeros.
+ * W1 the first `inter` rows of w13[e], W3 the others; sums in float32, h kept in 16 significant bits (two bfloat16 numbers).  A logit of
+ * -infinity takes an expert out: if it is among the topk all the same its weight is 0 and it adds nothing; a token with no other logits
+ * gets zeros.
  * weight_dtype KCG_DT_E4M3 (block scales; dtype KCG_DT_BFLOAT16 or KCG_DT_FLOAT16) or KCG_DT_BFLOAT16 (dtype the same).
  * hidden and inter are multiples of 16; experts <= 512, topk <= 16.
  * workspace: kcg_moe_workspace_bytes() bytes on 16, in use until the stream has passed the call. */
@@ -97,7 +98,7 @@ typedef struct kcg_moe_layer_args {
   int64_t ids, probs;      /* out: [tokens, topk] contiguous, int32 and float32, by falling logit */
   int64_t workspace, workspace_bytes;
   int64_t x_stride, logits_stride, out_stride;
-  int64_t w13_stride_expert, w13_stride_row, w2_stride_expert, w2_stride_row; /* bytes: multiples of 16 */
+  int64_t w13_stride_expert, w13_stride_row, w2_stride_expert, w2_stride_row; /* multiples of 16 bytes */
   int64_t tokens, experts, topk, hidden, inter, dtype, weight_dtype, renormalize;
 } kcg_moe_layer_args;
 int kcg_moe_layer(const kcg_moe_layer_args* args, int device, uint64_t stream);
