@@ -35,7 +35,8 @@ using namespace kcg_ops;
 // is smallest for: every round of blocks costs start + steps * step, where a round is one block on each of the 256 compute
 // units, or two where two fit one (step2: their step); steps = groups of 128 of K / ks.  Products with float32 results take
 // nearly twice the matrix instructions a step, so they have costs of their own.  Measured at N, K in {1024 .. 16384}; the
-// estimates lie within 10 % of what was measured, some 20 % at the largest sizes and between one round and two.
+// estimates lie within 10 % of what was measured, some 20 % at the largest sizes and between one round and two.  The figures beside
+// the tiles, and at the other choices below, are microseconds a call in a graph of calls, both sides on one card.
 struct Cost {
   float start, step, step2;
 };
@@ -45,16 +46,16 @@ struct Tile {
   Cost half, full;                                        // 16-bit results, float32 results
 };
 const Tile kTileTable[] = {
-    {"32x32_2x1x4", 32, 32, 4, 512, {1.6f, .39f, 0.f}, {1.9f, .64f, 0.f}},        // 37 x 4096 x 4096: 7.4 us (64 x 64: 12.4)
-    {"64x32_4x1x2", 64, 32, 2, 512, {1.2f, .36f, 0.f}, {1.4f, .62f, 0.f}},        // 37 x 8192 x 4096: 9.5 (32 x 32: 12.8, 64 x 64 by two: 10.8)
-    {"64x64_2x2x1", 64, 64, 1, 256, {.4f, .305f, .52f}, {1.2f, .52f, .74f}},      // 512 x 4096 x 1024: 7.2 (by two: 10.8)
-    {"64x64_2x2x2", 64, 64, 2, 512, {1.9f, .47f, 0.f}, {2.2f, .76f, 0.f}},        // 256 x 4096 x 4096: 11.3 (by one: 12.8)
-    {"64x128_2x2x1", 64, 128, 1, 256, {.8f, .6f, .67f}, {1.6f, .74f, 1.07f}},     // 4096 x 1536 x 1000, float32: 22.4 (64 x 64: 28.1, 128 x 128: 25.0)
-    {"128x128_2x2x1", 128, 128, 1, 256, {1.6f, .655f, 1.1f}, {4.6f, 1.08f, 1.75f}},  // 2048 x 4096 x 4096: 39.8 (8 waves: 45.7)
+    {"32x32_2x1x4", 32, 32, 4, 512, {1.6f, .39f, 0.f}, {1.9f, .64f, 0.f}},        // 37 x 4096 x 4096: 7.9 us (64 x 64: 12.9)
+    {"64x32_4x1x2", 64, 32, 2, 512, {1.2f, .36f, 0.f}, {1.4f, .62f, 0.f}},        // 37 x 8192 x 4096: 10.1 (32 x 32: 13.4, 64 x 64 by two: 11.3)
+    {"64x64_2x2x1", 64, 64, 1, 256, {.4f, .305f, .52f}, {1.2f, .52f, .74f}},      // 512 x 4096 x 1024: 7.8 (by two: 11.2)
+    {"64x64_2x2x2", 64, 64, 2, 512, {1.9f, .47f, 0.f}, {2.2f, .76f, 0.f}},        // 256 x 4096 x 4096: 12.2 (by one: 13.4)
+    {"64x128_2x2x1", 64, 128, 1, 256, {.8f, .6f, .67f}, {1.6f, .74f, 1.07f}},     // 4096 x 1536 x 1000, float32: 22.7 (64 x 64: 28.3, 128 x 128: 24.1)
+    {"128x128_2x2x1", 128, 128, 1, 256, {1.6f, .655f, 1.1f}, {4.6f, 1.08f, 1.75f}},  // 2048 x 4096 x 4096: 40.5 (8 waves: 46.9)
     // for 16-bit results only: the next two are no faster than 64 x 64 and 64 x 128 with float32 ones, the last has no registers for them
-    {"128x64_4x2x1", 128, 64, 1, 512, {.6f, .5f, 0.f}, {}},                       // 128 x 16384 x 4096: 23.0 (64 x 64: 27.0)
-    {"128x128_4x2x1", 128, 128, 1, 512, {2.f, .575f, 0.f}, {}},                   // 1024 x 4096 x 4096: 23.5 (4 waves: 28.0)
-    {"256x256_4x2x1", 256, 256, 1, 512, {7.f, 1.55f, 0.f}, {}},                   // 4096^3: 61.5 (128 x 128: 73.8)
+    {"128x64_4x2x1", 128, 64, 1, 512, {.6f, .5f, 0.f}, {}},                       // 128 x 16384 x 4096: 17.8 (64 x 64: 18.5)
+    {"128x128_4x2x1", 128, 128, 1, 512, {2.f, .575f, 0.f}, {}},                   // 1024 x 4096 x 4096: 24.3 (4 waves: 27.4)
+    {"256x256_4x2x1", 256, 256, 1, 512, {7.f, 1.55f, 0.f}, {}},                   // 4096^3: 64.7 (128 x 128: 91.3)
 };
 constexpr int kTiles = sizeof(kTileTable) / sizeof(kTileTable[0]), kTilesF32 = kTiles - 3;
 constexpr double kLaunch = 2.3;
@@ -99,7 +100,7 @@ MatmulChoice choose_matmul(int64_t m, int64_t n, int64_t k, int t) {
   const int64_t groups = (k + 127) / 128;
   int rt = 0, tile = 0;                    // rt > 0: without a tile
   if (m <= 16) {
-    rt = n >= 32 * 224 ? 2 : 1;            // 32 rows of b a block where that still fills the chip (8 x 8192 x 4096: 8.3 us, with 16 rows 9.5)
+    rt = n >= 32 * 224 ? 2 : 1;            // 32 rows of b a block where that still fills the chip (8 x 8192 x 4096: 8.6, with 16 rows 9.9)
   } else {
     double best = 1e30;
     for (int v = 0; v < (t == 2 ? kTilesF32 : kTiles); ++v) {
@@ -165,14 +166,15 @@ MoePlan moe_plan(int64_t tokens, int64_t experts, int64_t topk, int64_t hidden, 
   const int64_t pairs = tokens * topk, cols = (hidden + DOWN_MANY_COLS - 1) / DOWN_MANY_COLS;
   m.slots = pairs < experts ? pairs : experts;
   m.plane = pairs * inter * 2;
-  // 16 columns of out a block: with fewer blocks than compute units only the smallest calls gain (3 tokens, 2 of 8 experts of
-  // 4096 x 2048 in bf16: 63.7 us, the other way 50.5; 2 tokens, 8 of 128 experts of 1024 x 4096: 46.4, the other way 53)
+  // 16 columns of out a block: with fewer blocks than compute units only the smallest calls gain (2 tokens, 8 of 128 experts of
+  // 1024 x 4096: the call takes 48.2, the other way 52.9; 3 tokens, 2 of 8 of 4096 x 2048 in bf16, half as many blocks: 59.5, 59.4)
   m.few = tokens <= MOE_FEW && moe_h_bytes(pairs, inter) <= (hidden >= 16 * 256 ? MOE_H_LDS : MOE_H_LDS / 2);
   // one block on each of the 256 compute units; waves without an item of their own share I, in parts.  There are at least
   // `items` items: k experts, and `per` pairs an item.
   m.z = cols >= 256 ? 1 : (int)(256 / cols);
   // Items of 16 pairs halve the reads of W2 by experts of more than 8 tokens and cost the others four more loads a step: 64 tokens, 4 of 16
-  // experts of 2048 x 4096 48 us (by eight 57), 2 of 8 of 2048 x 4096 25 (27); 8 tokens an expert cost the same either way.
+  // experts of 2048 x 4096: the call takes 126.7 (by eight 137.7), 2 of 8 of the same 73.9 (78.8); 8 tokens an expert (8 of 64 of 1024 x
+  // 2048) cost nearly the same either way, 101.2 (103.7).
   m.per = pairs > 8 * experts ? 16 : 8;
   const int64_t items = std::max<int64_t>(std::max<int64_t>(topk, (pairs + m.per - 1) / m.per), 1);
   m.max_parts = (int)std::max<int64_t>(1, std::min<int64_t>(m.z * DOWN_MANY_WAVES / items, groups(inter)));
@@ -409,9 +411,9 @@ int kcg_moe_layer(const kcg_moe_layer_args* p, int device, uint64_t stream) {
                (void*)p->out, (int32_t*)p->ids, (float*)p->probs, ws, ws + m.plane, (float*)(ws + 2 * m.plane), (int*)(ws + m.parts_at), (float*)(ws + m.y_at),
                p->x_stride, p->logits_stride, p->out_stride, p->w13_stride_expert, p->w13_stride_row, p->w2_stride_expert, p->w2_stride_row,
                (int)p->tokens, (int)p->experts, (int)p->topk, (int)p->hidden, (int)p->inter, (int)m.slots, p->renormalize != 0, 2, m.max_parts};
-  // Waves that share 16 rows of the first product: as few as leave 4096 waves to the chip, two at least (at 64 tokens, 128
-  // experts of 1024 x 4096: 220 us with one, 196 with two, 215 with four, 260 with eight; at one token, 8 of 64 experts
-  // of 1024 x 2048: 23.2, 14.8, 10.4 and 9.9).
+  // Waves that share 16 rows of the first product: as few as leave 4096 waves to the chip, two at least (64 tokens, 8 of 128
+  // experts of 1024 x 4096: the call takes 339 with one, 303 with two, 326 with four, 365 with eight; one token, 8 of 64 experts
+  // of 1024 x 2048: 33.5, 24.4, 19.7 and 19.3).
   const int64_t row_groups = p->inter / 16;
   while (a.split < UP_WAVES && row_groups * m.slots * a.split < 4096) a.split *= 2;
   const int per_block = UP_WAVES / a.split;

@@ -210,7 +210,7 @@ struct F16Ops {
 // form does the same): at most 2^-10 of the sum of the magnitudes, 1.4e-5 of the result on normal data, where a 16-bit result's half step
 // is larger (bf16 2^-8, fp16 2^-11); where products cancel it may be all of the result, and it is above what a float32 result
 // promises.  WideDot: the same values as bf16, which holds them exactly, in four instructions of half the rate, with float32
-// sums.  Results in 16 bits take the first, for its rate (4096^3: 67 us, on the same card in float32 127), in 32 bits the second.
+// sums.  Results in 16 bits take the first, for its rate (4096^3: 65 us, on the same card in float32 130), in 32 bits the second.
 struct E4m3Dot {
   typedef i32x8 frag;
   static __device__ __forceinline__ frag make(i32x8 q) { return q; }

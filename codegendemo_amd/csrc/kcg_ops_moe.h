@@ -204,7 +204,7 @@ __device__ __forceinline__ int route(const MoeArgs& a, RouteLds& s, int slot, bo
 // grid (x, slots), UP_WAVES waves.  A row group is 16 gate rows and the 16 up rows beside them.  `split` waves share a row
 // group, each with a part of H, and meet in LDS; UP_WAVES / split row groups run side by side.  The loads of a step (a group of
 // 128 of one row group) are issued before the products of the step in front of it (up to 16 tokens).  Measured: 64 tokens, 8 of 128
-// experts of 1024 x 4096 in e4m3, 213 us (1.07 GB: 5.0 TB/s); a token, 8 of 64 of 1024 x 2048, 10.6 us, of which the weights' bytes are
+// experts of 1024 x 4096 in e4m3, 192 us (1.06 GB: 5.5 TB/s); a token, 8 of 64 of 1024 x 2048, 10.6 us, of which the weights' bytes are
 // 5.2 and the rest a launch, the routing and the first loads, one after another.
 template <class Ops, class W, class X, int CT>
 __device__ __forceinline__ void up_tiles(const MoeArgs& a, RouteLds& s, f32x4* red, int ex, int count, int skip) {
@@ -553,7 +553,7 @@ struct DownWave {
 
 // One token or a few whose h fits LDS: grid H / 16, a block makes 16 columns of every token's row.  The waves put their partial
 // sums side by side in LDS and the block adds them up.  Four steps of loads in flight.  A token, 8 of 64 experts of 1024 x 2048:
-// 9.0 us (12.7 with h from memory, 11.1 with h asked for behind the sorting).
+// 8.8 us (9.0 on the card where it took 12.7 with h from memory and 11.1 with h asked for behind the sorting).
 template <class W, class X>
 __device__ void down_few_kernel(const MoeArgs& a, float* partial) {
   __shared__ SortLds s;
@@ -608,7 +608,7 @@ __device__ void down_few_kernel(const MoeArgs& a, float* partial) {
 // More of them: grid (H / 64, z), a block makes 64 columns of the pairs of its share of the items, which go to memory as
 // y[part][pair][H] in 32 bits; combine_kernel adds them up.  Four tiles beside each other use a load of h four times: with one
 // (and all items in one block, no memory between) the loads' addresses took longer than the weights: 64 tokens, 8 of 128 experts
-// of 1024 x 4096 155 us, so 111 and 5 for the sum; 11 tokens, 2 of 8 of 4096 x 2048 in bf16 50, so 32 and 5.
+// of 1024 x 4096 155 us, so 106 and 5 for the sum; 11 tokens, 2 of 8 of 4096 x 2048 in bf16 50, so 29 and 5.
 template <class W, int PER>
 __device__ void down_many_kernel(const MoeArgs& a) {
   __shared__ SortLds s;

@@ -1,7 +1,7 @@
 // kcg_ops_quant.h — the two operators that make 8-bit operands: root-mean-square norm with the residual's addition, and the
 // gated activation.  Both are bound by memory: one pass, 16-byte accesses, the row in registers between the sum and its use.
-// Measured: norm with residual and y, 8192 x 4096 bf16, 55.5 us (5.46 TB/s; a copy reaches 5.06); one row 2.5 us, which is
-// a launch and two latencies; activation, 4096 x 8192 bf16, 32.4 us (5.2 TB/s), 16 x 4096 2.6 us.
+// Measured: norm with residual and y, 8192 x 4096 bf16, 55.7 us (5.44 TB/s; a copy reaches 5.06); one row 2.6 us, which is
+// a launch and two latencies; activation, 4096 x 8192 bf16, 31.8 us (5.3 TB/s), 16 x 4096 2.6 us.
 #pragma once
 #include "kcg_ops_common.h"
 
@@ -115,7 +115,7 @@ __device__ void norm_kernel(const NormArgs& a) {
 }
 
 // h = gate / (1 + exp(-gate)) * up, quantised; 16 lanes a group, a thread 8 values.  (With expf and a division, 35 vector
-// instructions a value, it was bound by them: 37.5 us at 4096 x 8192, where silu_times takes 32.4.)
+// instructions a value, it was bound by them: 37.5 us at 4096 x 8192, on the same card 32.4 with silu_times.)
 template <class T>
 __device__ void swiglu_kernel(const SwigluArgs& a) {
   const unsigned per_row = (unsigned)((a.cols + GROUP - 1) / GROUP) * 16u;

@@ -1,7 +1,7 @@
 // kcg_torch.cc — the operators of the 8-bit path on torch tensors: checks of the arguments, outputs, the call.
 // A small call is over in 3 to 5 us on the GPU, and the runtime's launch takes the host 3.1; with the same steps in Python a
 // call took the host 7.4 to 8.5 us (an output 1.3, a checked operand 0.5), so a decoded token waited for it.  Here a whole call
-// takes 4.3 to 4.7 us (moe_layer, of two or three launches: 8.5, 11).
+// takes 3.1 to 3.5 us with the caller's outputs, 3.8 to 4.7 where one or two are made (moe_layer, of two or three launches: 8.6, 11.3).
 //
 // The module links neither the library nor a HIP runtime: bind() gives it the addresses of the C entry points
 // (include/kcg_ops.h), so that both bindings run the one library that the process has loaded.
